@@ -38,6 +38,13 @@ SIGNATURES = {
     "hific_channelnorm_fwd_exact_res": (I, [P, P, P, P, I, P, P, P, P, P, I, I, I, F, I, I, P]),
     "hific_channelnorm_bwd_ws_bytes": (Z, [I, I, I]),
     "hific_channelnorm_bwd": (I, [P] * 9 + [I, I, I, I, I, I, P, Z, P, I, P]),
+    "hific_act8_pack": (I, [P, P, P] + [I] * 5 + [P]),
+    "hific_act8_restore": (I, [P, P, I, P, P, I, P] + [I] * 4 + [P]),
+    "hific_rms_norm_fwd": (I, [P] * 8 + [I] * 5 + [F, I, P]),
+    "hific_norm8_bwd_ws_bytes": (Z, [I, I, I]),
+    "hific_rms_norm_bwd": (I, [P, P, P, I] + [P] * 6 + [I] * 5 + [P, Z, P]),
+    "hific_channelnorm8_fwd": (I, [P] * 10 + [I] * 4 + [F, I, I, P]),
+    "hific_channelnorm8_bwd": (I, [P, P, I] + [P] * 7 + [I, P] + [I] * 6 + [P, Z, P]),
     "hific_act_bwd": (I, [P, P, P, L, F, I, P]),
     "hific_tanh_fwd": (I, [P, P, L, I, P]),
     "hific_tanh_bwd": (I, [P, P, P, L, I, P]),

@@ -2115,3 +2115,9 @@ def hyper_symbols_and_indices(hyperlatents):
     idx = torch.empty(z.shape, dtype=torch.int32, device=z.device)
     call("hific_hyper_symbols", ptr(z), ptr(sym), ptr(idx), N, C, H * W, stream())
     return sym, idx
+
+
+# ------------------------------------------------------------------------------------------------------
+# activations in 8 bits, the norms that write and read them, root-mean-square norm (act8.py)
+from .act8 import (Act8, checkpoint8, restore8, rms_norm, rms_norm8, channel_norm8, channel_norm_grad8,  # noqa: E402,F401
+                   conv2d_weight_grad8, conv_transpose2d_weight_grad8)

@@ -134,6 +134,42 @@ int hific_channelnorm_bwd(const void* x, const void* dy, const float* gamma, con
                           int accumulate, int dtype, void* ws, size_t ws_bytes, float* dprev_bias, int accumulate_prev,
                           hipStream_t stream);
 
+/* ---- activations in 8 bits (csrc/act8.hip), norms that write or read them, root-mean-square norm (csrc/norm8.hip) ----------
+ * No counterpart in the reference: its training keeps every activation in float32 (autograd of src/network/generator.py:145-168).
+ * A token is one position of an activation [N, C, HW] (HW = 1: rows).  q [N, C, HW] bytes: int8 (fmt 0) or e4m3 (fmt 1: finite
+ * only, largest value 448); qe [N, HW] bytes: exponent + 127.  value = q * 2^(qe - 127), qe the smallest exponent with
+ * max|v| <= QMAX * 2^(qe - 127) over the token's C values, QMAX = 127 or 448.  qe = 255: the token held an infinity or NaN and
+ * restores to NaN.  All tensors contiguous; no alignment is needed (16-byte aligned pointers and HW % 8 == 0, or HW = 1 and
+ * C % 8 == 0, reach the wide kernels).  x, y, resid, dy, ... are of `dtype`; weights, statistics and their gradients float32. */
+#define HIFIC_Q_INT8 0
+#define HIFIC_Q_E4M3 1
+int hific_act8_pack(const void* x, void* q, void* qe, int fmt, int N, int C, int HW, int dtype, hipStream_t stream);
+/* out = q * 2^e, or relu?(gamma_c * (q * 2^e) + beta_c) where gamma / beta (both or neither) are given */
+int hific_act8_restore(const void* q, const void* qe, int fmt, const float* gamma, const float* beta, int relu, void* out,
+                       int N, int C, int HW, int dtype, hipStream_t stream);
+/* h = x + resid (rounded to dtype; resid and h both or neither), rstd = rsqrt(mean_c h^2 + eps), xh = h * rstd, y = w_c * xh.
+ * y, rstd nullable; q / qe nullable (y or q is needed): xh in 8 bits, or y where q_of_y is set. */
+int hific_rms_norm_fwd(const void* x, const void* resid, const float* w, void* y, void* h, float* rstd, void* q, void* qe,
+                       int fmt, int q_of_y, int N, int C, int HW, float eps, int dtype, hipStream_t stream);
+/* workspace of the two backward entry points below */
+size_t hific_norm8_bwd_ws_bytes(int N, int C, int HW);
+/* from h (dtype) or, with h NULL, from xh in 8 bits.  dx = rstd * (g - xh * mean_c(g * xh)) + dstream, g = w * dy (dstream: the
+ * gradient that reaches h past the norm, nullable); dw (=|+= by accumulate) sum over tokens of dy * xh.  Fixed summation order. */
+int hific_rms_norm_bwd(const void* h, const void* q, const void* qe, int fmt, const float* rstd, const void* dy,
+                       const void* dstream, const float* w, void* dx, float* dw, int accumulate, int N, int C, int HW, int dtype,
+                       void* ws, size_t ws_bytes, hipStream_t stream);
+/* hific_channelnorm_fwd (src/normalisation/channel.py:48-59) that also writes what the backward pass needs in 8 bits: q / qe =
+ * the normalised xh (with relu: rounded to the side of the ReLU that xh is on), rstd.  y = relu?(gamma * xh + beta) (+ resid);
+ * q2 / qe2 (nullable, with resid): y in 8 bits, for the weight gradient of the convolution behind. */
+int hific_channelnorm8_fwd(const void* x, const float* gamma, const float* beta, const void* resid, void* y, float* rstd,
+                           void* q, void* qe, void* q2, void* qe2, int fmt, int N, int C, int HW, float eps, int relu, int dtype,
+                           hipStream_t stream);
+/* its backward pass from q / qe / rstd; dprev_bias as in hific_channelnorm_bwd */
+int hific_channelnorm8_bwd(const void* q, const void* qe, int fmt, const float* rstd, const void* dy, const float* gamma,
+                           const float* beta, void* dx, float* dgamma, float* dbeta, int accumulate, float* dprev_bias,
+                           int accumulate_prev, int N, int C, int HW, int relu, int dtype, void* ws, size_t ws_bytes,
+                           hipStream_t stream);
+
 /* ---- elementwise / reductions (csrc/elementwise.hip) -------------------------------------------------------- */
 /* dx = y>0 ? dy : slope*dy — backward of F.relu (src/network/hyper.py:59-60,91-92) / LeakyReLU */
 int hific_act_bwd(const void* dy, const void* y, void* dx, long long n, float slope, int dtype, hipStream_t stream);
