@@ -20,6 +20,7 @@ typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 // |v| as unsigned bits: ordered like the magnitudes, infinities above every number and NaN above those (fmaxf would lose a NaN)
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned umin(unsigned a, unsigned b) { return a < b ? a : b; }
 
 // amax as abs_bits -> the byte of the exponent.  QMAX = 1.984375 * 2^6 (127) or 1.75 * 2^8 (448).
 template <int FMT>
@@ -78,6 +79,199 @@ __device__ __forceinline__ unsigned q8_round_masked(float xh, float inv, float s
     if ((fmaf(gamma, v * scale, beta) > 0.f) != (fmaf(gamma, xh, beta) > 0.f)) b = q8_next<FMT>(b, t > v);
     return b;
 }
+
+// ---- eight values at a time ------------------------------------------------------------------------------------------------
+// The wide kernels give a lane eight neighbouring values (16 bytes of bfloat16): of a plane (eight positions of a channel) or of a
+// row (eight channels of a token).  The types are aligned to one element only, so odd planes and rows take the same path
+// (gfx950 loads and stores 16 bytes at any address); a last group of fewer than eight is moved back to end at the plane's or row's
+// end, and its first values are then computed twice, with the same result.
+typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
+typedef u32x2_t u32x2_a1 __attribute__((aligned(1)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+template <typename T> struct V8;
+template <> struct V8<bf16_t> {
+    u32x4_t r;
+    __device__ __forceinline__ void load(const bf16_t* p) { r = *(const u32x4_a2*)p; }
+    __device__ __forceinline__ float get(int j) const { return __uint_as_float((j & 1) ? (r[j >> 1] & 0xffff0000u) : (r[j >> 1] << 16)); }
+    __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = f2bf2(v[2 * j], v[2 * j + 1]);
+    }
+    __device__ __forceinline__ void store(bf16_t* p) const { *(u32x4_a2*)p = r; }
+};
+template <> struct V8<float> {
+    f32x4_a4 r[2];
+    __device__ __forceinline__ void load(const float* p) { r[0] = *(const f32x4_a4*)p; r[1] = *(const f32x4_a4*)(p + 4); }
+    __device__ __forceinline__ float get(int j) const { return r[j >> 2][j & 3]; }
+    __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j >> 2][j & 3] = v[j];
+    }
+    __device__ __forceinline__ void store(float* p) const { *(f32x4_a4*)p = r[0]; *(f32x4_a4*)(p + 4) = r[1]; }
+};
+
+// eight values, already divided by their scales -> eight bytes.  CLAMP: only where |t| can exceed QMAX by a rounding (see q8_round).
+template <int FMT, bool CLAMP>
+__device__ __forceinline__ u32x2_t q8_pack8(const float* t) {
+    u32x2_t o;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float m = FMT == HIFIC_Q_INT8 ? 127.f : 448.f;
+            v[j] = CLAMP ? __builtin_amdgcn_fmed3f(t[4 * h + j], -m, m) : t[4 * h + j];
+        }
+        if (FMT == HIFIC_Q_INT8) {
+            unsigned b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(v[j] + 12582912.f);
+            o[h] = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+        } else {
+            int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+            o[h] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+        }
+    }
+    return o;
+}
+// eight bytes -> eight numbers, without the exponents
+template <int FMT>
+__device__ __forceinline__ void q8_unpack8(u32x2_t q, float* v) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (FMT == HIFIC_Q_INT8) {
+            const unsigned u = q[h] ^ 0x80808080u;               // unsigned bytes convert in one instruction each
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * h + j] = (float)((u >> (8 * j)) & 0xffu) - 128.f;
+        } else {
+            const hw_f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
+            v[4 * h] = a[0]; v[4 * h + 1] = a[1]; v[4 * h + 2] = b[0]; v[4 * h + 3] = b[1];
+        }
+    }
+}
+
+// eight normalised values whose ReLU follows (v = gamma xh + beta): q8_round_masked of each.  Without the clamp: max|xh| gave the
+// exponent, so |xh * inv| <= QMAX.
+template <int FMT>
+__device__ __forceinline__ u32x2_t q8_pack8_masked(const float* xh, const float* inv, const float* v, float gamma, float beta) {
+    if (FMT == HIFIC_Q_INT8) {
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = xh[j] * inv[j], n = rintf(x);
+            const float scale = __uint_as_float(0x7f000000u - __float_as_uint(inv[j]));      // 1 / inv, a power of two
+            const bool wrong = (fmaf(gamma, n * scale, beta) > 0.f) != (v[j] > 0.f);
+            t[j] = wrong ? n + (x > n ? 1.f : -1.f) : n;
+        }
+        return q8_pack8<FMT, true>(t);
+    }
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = xh[j] * inv[j];
+    u32x2_t q = q8_pack8<FMT, false>(t);
+    float n[8];
+    q8_unpack8<FMT>(q, n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float scale = __uint_as_float(0x7f000000u - __float_as_uint(inv[j]));
+        if ((fmaf(gamma, n[j] * scale, beta) > 0.f) != (v[j] > 0.f)) {
+            const int sh = 8 * (j & 3);
+            const unsigned b = q8_next<FMT>((q[j >> 2] >> sh) & 0xffu, t[j] > n[j]);
+            q[j >> 2] = (q[j >> 2] & ~(0xffu << sh)) | (b << sh);
+        }
+    }
+    return q;
+}
+__device__ __forceinline__ float relu_nan(float v) { return v > 0.f || v != v ? v : 0.f; }
+
+// Planes: lane = (group of eight positions pl = lane % LPX, channel sub-group lane / LPX).  v[j], this lane's partial of position j,
+// is combined over the 64 / LPX sub-groups of the wave: the first three steps exchange halves (4 + 2 + 1 shuffles where eight
+// separate butterflies would take 8 per step), the rest, if any, carry one value.  out[pl * 8 + j] receives the wave's result.
+template <int LPX, bool MAX, typename V>
+__device__ __forceinline__ void tile_reduce(const V* v, V* out) {
+    const int lane = threadIdx.x & 63, sub = lane / LPX;
+    auto shfl = [](V x, int o) { return __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(int, x), o, 64)); };
+    auto op = [](V x, V y) { return MAX ? (x > y ? x : y) : x + y; };
+    const bool b0 = sub & 1, b1 = sub & 2, b2 = sub & 4;
+    V a[4], c[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = op(b0 ? v[4 + j] : v[j], shfl(b0 ? v[j] : v[4 + j], LPX));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) c[j] = op(b1 ? a[2 + j] : a[j], shfl(b1 ? a[j] : a[2 + j], 2 * LPX));
+    V d = op(b2 ? c[1] : c[0], shfl(b2 ? c[0] : c[1], 4 * LPX));
+#pragma unroll
+    for (int o = 8 * LPX; o < 64; o <<= 1) d = op(d, shfl(d, o));
+    if (sub < 8) out[(lane % LPX) * 8 + (b0 ? 4 : 0) + (b1 ? 2 : 0) + (b2 ? 1 : 0)] = d;
+}
+
+// Workgroups go round-robin to the 8 XCDs, each with its own L2; neighbouring tiles share 128-byte lines where a tile is narrower
+// than 64 positions: hand each XCD a contiguous range of them.
+__device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
+    return (total & 7u) == 0 ? (bid & 7u) * (total >> 3) + (bid >> 3) : bid;
+}
+
+// Tile of the plane kernels: 256 threads, LPX groups of eight positions, 256 / LPX channel groups, at most `most` channels per
+// thread.  The widest LPX (8: whole 128-byte lines) that fits the channels, then narrower while the grid would not fill the
+// 256 CUs twice and a thread has more than one channel.  lpx = 0: more channels than the registers hold.
+struct TileCfg { int lpx, cpt; unsigned tiles; long long blocks; };
+static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
+    TileCfg t{0, 0, 0, 0};
+    for (int lpx = 8; lpx >= 1; lpx >>= 1) {
+        const int cpt = cdiv(C, 256 / lpx);
+        if (cpt > most) continue;
+        t.lpx = lpx; t.cpt = cpt;
+        t.tiles = (unsigned)cdiv(cdiv(HW, 8), lpx);
+        t.blocks = (long long)t.tiles * N;
+        if (t.blocks >= 512 || cpt <= 1) break;
+    }
+    return t;
+}
+
+// Rows: L lanes and K groups of eight channels per lane hold a row.  Sums and maxima over the row's L lanes, through LDS where a
+// row has the whole workgroup.
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+    for (int o = (L < 64 ? L : 64) >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (L == 256) {
+        __shared__ float red[4];
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    return v;
+}
+template <int L>
+__device__ __forceinline__ unsigned row_max(unsigned v) {
+#pragma unroll
+    for (int o = (L < 64 ? L : 64) >> 1; o > 0; o >>= 1) v = umax(v, (unsigned)__shfl_xor((int)v, o, 64));
+    if (L == 256) {
+        __shared__ unsigned red[4];
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = umax(umax(red[0], red[1]), umax(red[2], red[3]));
+    }
+    return v;
+}
+// 16 lanes for up to 128 channels, a wave for more, the whole workgroup for wide rows and where fewer than 1024 rows would leave
+// the other CUs idle.  l = 0: more channels than the registers hold.
+struct RowCfg { int l, k; };
+static inline RowCfg row_pick(long long N, int C) {
+    RowCfg r;
+    r.l = C <= 128 ? 16 : ((C > 2048 || (N < 1024 && C > 512)) ? 256 : 64);
+    r.k = cdiv(C, 8 * r.l);
+    if (r.k > 4) r.l = 0;
+    return r;
+}
+#define ROW_DISPATCH(r, F)                                                                              \
+    do {                                                                                                \
+        if ((r).l == 16) F(16, 1);                                                                      \
+        else if ((r).l == 64) { if ((r).k <= 1) F(64, 1); else if ((r).k <= 2) F(64, 2); else F(64, 4); } \
+        else if ((r).k <= 1) F(256, 1); else if ((r).k <= 2) F(256, 2); else F(256, 4);                 \
+    } while (0);
 
 static inline bool act8_dtype_ok(int dtype) { return dtype == HIFIC_F32 || dtype == HIFIC_BF16; }
 static inline bool act8_fmt_ok(int fmt) { return fmt == HIFIC_Q_INT8 || fmt == HIFIC_Q_E4M3; }

@@ -2,7 +2,7 @@
 // writes 1 byte per element, restore the reverse.
 #include "act8.h"
 
-// PX lanes on consecutive positions x 256 / PX channel groups; see norm8.hip for the choice of PX.
+// Any shape: PX lanes on consecutive positions x 256 / PX channel groups, the tensor read twice (the second time from L2).
 template <typename T, int FMT, int PX>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                         int C, int HW, unsigned tiles) {
@@ -24,56 +24,217 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x,
     for (int c = g; c < C; c += G) q[base + (size_t)c * HW] = (u8_t)q8_round<FMT>(DT<T>::ld(x + base + (size_t)c * HW) * inv);
 }
 
-// out = relu?(gamma_c * (q * 2^e) + beta_c), or q * 2^e where gamma is null
-template <typename T, int FMT>
-__global__ __launch_bounds__(256) void act8_restore_kernel(const u8_t* __restrict__ q, const u8_t* __restrict__ qe,
-                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                           T* __restrict__ out, int C, int HW, long long n, int relu) {
-    const long long step = (long long)gridDim.x * 256;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-        const long long plane = i / HW, img = plane / C;
-        float v = q8_value<FMT>(q[i]) * q8_scale(qe[img * HW + (i - plane * HW)]);
-        if (gamma) {
-            const int c = (int)(plane - img * C);
-            v = fmaf(gamma[c], v, beta[c]);
-            if (relu) v = v > 0.f ? v : (v != v ? v : 0.f);
+// Planes of eight positions and more: the tile stays in registers between the maximum and the rounding, one pass over HBM.
+template <typename T, int FMT, int LPX, int CPT>
+__global__ __launch_bounds__(256) void act8_pack_tile_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
+                                                             int C, int HW, unsigned tiles, unsigned blocks) {
+    constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
+    __shared__ unsigned red[4][TP];
+    __shared__ float inv_s[TP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
+    const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / tiles, tile = bid - n * tiles;
+    const unsigned oct = tile * LPX + pl, octs = ((unsigned)HW + 7) >> 3;
+    const bool ok = oct < octs;
+    const unsigned hw0 = umin(ok ? oct * 8 : 0u, (unsigned)HW - 8);
+    const size_t base = (size_t)n * C * HW + hw0;
+    V8<T> xr[CPT];
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) { const int c = g + G * k; xr[k].load(x + base + (size_t)(c < C ? c : 0) * HW); }
+    unsigned am[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) am[j] = 0;
+#pragma unroll
+    for (int k = 0; k < CPT; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) am[j] = umax(am[j], g + G * k < C ? abs_bits(xr[k].get(j)) : 0u);
+    tile_reduce<LPX, true>(am, red[wave]);
+    __syncthreads();
+    if (tid < TP) {
+        const unsigned code = q8_code<FMT>(umax(umax(red[0][tid], red[1][tid]), umax(red[2][tid], red[3][tid])));
+        inv_s[tid] = q8_inv_scale(code);
+        const unsigned o = tile * LPX + (tid >> 3);
+        if (o < octs) qe[(size_t)n * HW + umin(o * 8, (unsigned)HW - 8) + (tid & 7)] = (u8_t)code;
+    }
+    __syncthreads();
+    float inv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) inv[j] = inv_s[pl * 8 + j];
+    if (!ok) return;
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int c = g + G * k;
+        if (c < C) {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = xr[k].get(j) * inv[j];
+            *(u32x2_a1*)(q + base + (size_t)c * HW) = q8_pack8<FMT, false>(t);
         }
-        DT<T>::st(out + i, v);
     }
 }
+
+// out = relu?(gamma_c * (q * 2^e) + beta_c), or q * 2^e where gamma is null.  V positions x CH channels per thread: the exponents
+// are read once for CH channels.  V = 8 for planes of eight positions and more; V = 1 otherwise (rows of odd shape, tiny planes).
+template <typename T, int FMT, int V, int CH>
+__global__ __launch_bounds__(256) void act8_restore_kernel(const u8_t* __restrict__ q, const u8_t* __restrict__ qe,
+                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                           T* __restrict__ out, int C, int HW, unsigned octs, unsigned cgs, long long n,
+                                                           int relu) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const long long rest = i / octs;
+    const unsigned oct = (unsigned)(i - rest * octs);
+    const long long img = rest / cgs;
+    const int c0 = (int)(rest - img * cgs) * CH;
+    const unsigned hw0 = V == 1 ? oct : umin(oct * 8, (unsigned)HW - 8);
+    const size_t base = ((size_t)img * C + c0) * HW + hw0;
+    float s[V];
+    if constexpr (V == 8) {
+        const u32x2_t e = *(const u32x2_a1*)(qe + (size_t)img * HW + hw0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = q8_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
+    } else s[0] = q8_scale(qe[(size_t)img * HW + hw0]);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+        if (c0 + k >= C) break;
+        float v[V];
+        if constexpr (V == 8) q8_unpack8<FMT>(*(const u32x2_a1*)(q + base + (size_t)k * HW), v);
+        else v[0] = q8_value<FMT>(q[base + (size_t)k * HW]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            v[j] *= s[j];
+            if (gamma) {
+                v[j] = fmaf(gamma[c0 + k], v[j], beta[c0 + k]);
+                if (relu) v[j] = relu_nan(v[j]);
+            }
+        }
+        if constexpr (V == 8) { V8<T> o; o.set(v); o.store(out + base + (size_t)k * HW); }
+        else DT<T>::st(out + base + (size_t)k * HW, v[0]);
+    }
+}
+
+// Rows (HW = 1) of eight channels and more: eight channels per lane, L lanes and K groups per lane for a row.
+template <typename T, int FMT, int L, int K>
+__global__ __launch_bounds__(256) void act8_pack_rows_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe, int N, int C) {
+    const int l = threadIdx.x % L;
+    const long long row0 = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const bool ok = row0 < N;
+    const size_t base = (size_t)(ok ? row0 : N - 1) * C;
+    V8<T> xr[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) xr[k].load(x + base + umin((unsigned)(l + L * k) * 8, (unsigned)C - 8));
+    unsigned am = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) am = umax(am, abs_bits(xr[k].get(j)));
+    am = row_max<L>(am);
+    const unsigned code = q8_code<FMT>(am);
+    const float inv = q8_inv_scale(code);
+    if (!ok) return;
+    if (l == 0) qe[row0] = (u8_t)code;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned c = (unsigned)(l + L * k) * 8;
+        if (c < (unsigned)C) {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = xr[k].get(j) * inv;
+            *(u32x2_a1*)(q + base + umin(c, (unsigned)C - 8)) = q8_pack8<FMT, false>(t);
+        }
+    }
+}
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void act8_restore_rows_kernel(const u8_t* __restrict__ q, const u8_t* __restrict__ qe,
+                                                                const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                                T* __restrict__ out, int C, unsigned octs, long long n, int relu) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const long long row = i / octs;
+    const unsigned c = umin((unsigned)(i - row * octs) * 8, (unsigned)C - 8);
+    const float s = q8_scale(qe[row]);
+    float v[8];
+    q8_unpack8<FMT>(*(const u32x2_a1*)(q + (size_t)row * C + c), v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] *= s;
+        if (gamma) {
+            v[j] = fmaf(gamma[c + j], v[j], beta[c + j]);
+            if (relu) v[j] = relu_nan(v[j]);
+        }
+    }
+    V8<T> o; o.set(v); o.store(out + (size_t)row * C + c);
+}
+
+namespace {
+template <typename T, int FMT>
+int pack_launch(const T* x, u8_t* q, u8_t* qe, int N, int C, int HW, hipStream_t st) {
+    if (HW >= 8) {
+        const TileCfg t = tile_pick(N, C, HW, 8);
+        if (t.lpx) {
+            if (t.blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
+            const dim3 grid((unsigned)t.blocks);
+#define TILE(LPX, CPT) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT>), grid, dim3(256), 0, st, x, q, qe, C, HW, t.tiles, (unsigned)t.blocks)
+#define TILE_C(LPX) do { if (t.cpt <= 1) TILE(LPX, 1); else if (t.cpt <= 2) TILE(LPX, 2); else if (t.cpt <= 4) TILE(LPX, 4); else TILE(LPX, 8); } while (0)
+            if (t.lpx == 8) TILE_C(8); else if (t.lpx == 4) TILE_C(4); else if (t.lpx == 2) TILE_C(2); else TILE_C(1);
+#undef TILE_C
+#undef TILE
+            return hific_launch_status();
+        }
+    }
+    RowCfg r;
+    if (HW == 1 && C >= 8 && (r = row_pick(N, C)).l) {
+#define ROWS(L, K) hipLaunchKernelGGL((act8_pack_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, 256 / L)), dim3(256), 0, st, x, q, qe, N, C)
+        ROW_DISPATCH(r, ROWS)
+#undef ROWS
+        return hific_launch_status();
+    }
+    const int px = HW == 1 ? 1 : (HW < 48 ? 16 : 64);
+    const long long tiles = cdivl(HW, px), blocks = tiles * N;
+    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)blocks);
+    if (px == 1) hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 1>), grid, dim3(256), 0, st, x, q, qe, C, HW, (unsigned)tiles);
+    else if (px == 16) hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 16>), grid, dim3(256), 0, st, x, q, qe, C, HW, (unsigned)tiles);
+    else hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 64>), grid, dim3(256), 0, st, x, q, qe, C, HW, (unsigned)tiles);
+    return hific_launch_status();
+}
+
+template <typename T, int FMT>
+int restore_launch(const u8_t* q, const u8_t* qe, const float* gamma, const float* beta, int relu, T* out, int N, int C, int HW, hipStream_t st) {
+    if (HW == 1 && C >= 8) {
+        const unsigned octs = (unsigned)cdiv(C, 8);
+        const long long n = (long long)octs * N, blocks = cdivl(n, 256);
+        if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
+        hipLaunchKernelGGL((act8_restore_rows_kernel<T, FMT>), dim3((unsigned)blocks), dim3(256), 0, st, q, qe, gamma, beta, out, C, octs, n, relu);
+        return hific_launch_status();
+    }
+    constexpr int CH = 4;
+    const unsigned octs = HW >= 8 ? (unsigned)cdiv(HW, 8) : (unsigned)HW, cgs = (unsigned)cdiv(C, CH);
+    const long long n = (long long)octs * cgs * N, blocks = cdivl(n, 256);
+    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
+    if (HW >= 8) hipLaunchKernelGGL((act8_restore_kernel<T, FMT, 8, CH>), dim3((unsigned)blocks), dim3(256), 0, st, q, qe, gamma, beta, out, C, HW, octs, cgs, n, relu);
+    else hipLaunchKernelGGL((act8_restore_kernel<T, FMT, 1, CH>), dim3((unsigned)blocks), dim3(256), 0, st, q, qe, gamma, beta, out, C, HW, octs, cgs, n, relu);
+    return hific_launch_status();
+}
+}  // namespace
 
 extern "C" {
 
 int hific_act8_pack(const void* x, void* q, void* qe, int fmt, int N, int C, int HW, int dtype, hipStream_t st) {
     if (!x || !q || !qe || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
-    const int px = HW == 1 ? 1 : (HW < 48 ? 16 : 64);
-    const long long tiles = cdivl(HW, px), blocks = tiles * N;
-    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-#define PACK(T, F, PX) hipLaunchKernelGGL((act8_pack_kernel<T, F, PX>), dim3((unsigned)blocks), dim3(256), 0, st, (const T*)x, \
-                                          (u8_t*)q, (u8_t*)qe, C, HW, (unsigned)tiles)
-#define PACK_P(T, F) do { if (px == 1) PACK(T, F, 1); else if (px == 16) PACK(T, F, 16); else PACK(T, F, 64); } while (0)
-#define PACK_F(T) do { if (fmt == HIFIC_Q_INT8) PACK_P(T, HIFIC_Q_INT8); else PACK_P(T, HIFIC_Q_E4M3); } while (0)
-    if (dtype == HIFIC_F32) PACK_F(float); else PACK_F(bf16_t);
-#undef PACK_F
-#undef PACK_P
+#define PACK(T) (fmt == HIFIC_Q_INT8 ? pack_launch<T, HIFIC_Q_INT8>((const T*)x, (u8_t*)q, (u8_t*)qe, N, C, HW, st) \
+                                     : pack_launch<T, HIFIC_Q_E4M3>((const T*)x, (u8_t*)q, (u8_t*)qe, N, C, HW, st))
+    return dtype == HIFIC_F32 ? PACK(float) : PACK(bf16_t);
 #undef PACK
-    return hific_launch_status();
 }
 
 int hific_act8_restore(const void* q, const void* qe, int fmt, const float* gamma, const float* beta, int relu, void* out,
                        int N, int C, int HW, int dtype, hipStream_t st) {
     if (!q || !qe || !out || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
     if ((gamma == nullptr) != (beta == nullptr) || (relu && !gamma)) return HIFIC_ERR_ARG;
-    const long long n = (long long)N * C * HW;
-    const long long want = cdivl(n, 256);
-    const unsigned blocks = (unsigned)(want < 65536 ? want : 65536);
-#define REST(T, F) hipLaunchKernelGGL((act8_restore_kernel<T, F>), dim3(blocks), dim3(256), 0, st, (const u8_t*)q,           \
-                                      (const u8_t*)qe, gamma, beta, (T*)out, C, HW, n, relu)
-#define REST_F(T) do { if (fmt == HIFIC_Q_INT8) REST(T, HIFIC_Q_INT8); else REST(T, HIFIC_Q_E4M3); } while (0)
-    if (dtype == HIFIC_F32) REST_F(float); else REST_F(bf16_t);
-#undef REST_F
+#define REST(T) (fmt == HIFIC_Q_INT8 ? restore_launch<T, HIFIC_Q_INT8>((const u8_t*)q, (const u8_t*)qe, gamma, beta, relu, (T*)out, N, C, HW, st) \
+                                     : restore_launch<T, HIFIC_Q_E4M3>((const u8_t*)q, (const u8_t*)qe, gamma, beta, relu, (T*)out, N, C, HW, st))
+    return dtype == HIFIC_F32 ? REST(float) : REST(bf16_t);
 #undef REST
-    return hific_launch_status();
 }
 
 }  // extern "C"

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p) {
         if (FMT != Q_NONE && ok)
             p.q[base + c * cs] = (u8_t)(MODE == M_CHAN && p.relu ? q8_round_masked<F>(xh, inv, scale, p.w[c], p.b[c])
                                                                  : q8_round<F>((MODE == M_RMS && p.q_of_y ? o : xh) * inv));
-        if (MODE == M_CHAN && p.relu) o = o > 0.f || o != o ? o : 0.f;
+        if (MODE == M_CHAN && p.relu) o = relu_nan(o);
         if (MODE == M_CHAN && rs) {      // both terms rounded to the storage type first, as norm and add one after the other
             T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
         }
@@ -111,10 +111,228 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p) {
         if (ok && g == 0) p.qe2[tok] = (u8_t)code2;
         for (int c = g; c < p.C; c += G) {
             float o = fmaf(p.w[c], (stream(c) - mu) * r, p.b[c]);
-            if (p.relu) o = o > 0.f || o != o ? o : 0.f;
+            if (p.relu) o = relu_nan(o);
             T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
             if (ok) p.q2[base + c * cs] = (u8_t)q8_round<F>(o * inv2);
         }
+    }
+}
+
+// Planes of eight positions and more: a workgroup owns LPX * 8 positions x all channels (tile_pick), eight positions and CPT
+// channels per lane, kept as they were loaded between the passes: every tensor crosses HBM once.
+template <typename T, int MODE, int FMT, int LPX, int CPT>
+__global__ __launch_bounds__(256) void norm8_fwd_tile_kernel(const NormFwd p, unsigned blocks) {
+    constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
+    constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;
+    __shared__ float red[4][TP];
+    __shared__ unsigned redm[4][TP];
+    __shared__ float st_r[TP], st_inv[TP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
+    const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / p.tiles, tile = bid - n * p.tiles;
+    const unsigned oct = tile * LPX + pl, octs = ((unsigned)p.HW + 7) >> 3;
+    const bool ok = oct < octs;
+    const size_t base = (size_t)n * p.C * p.HW + umin(ok ? oct * 8 : 0u, (unsigned)p.HW - 8);
+    // position tid of the tile, for the threads that finish the statistics
+    const unsigned so = tile * LPX + (tid >> 3);
+    const bool sok = tid < TP && so < octs;
+    const size_t stok = (size_t)n * p.HW + umin(so * 8, (unsigned)p.HW - 8) + (tid & 7);
+    const T* x = (const T*)p.x + base;
+    const T* rs = p.resid ? (const T*)p.resid + base : nullptr;
+    V8<T> xr[CPT], rr[MODE == M_CHAN ? CPT : 1];
+    float w[CPT], b[MODE == M_CHAN ? CPT : 1];
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int c = g + G * k, ci = c < p.C ? c : 0;
+        xr[k].load(x + (size_t)ci * p.HW);
+        w[k] = p.w[ci];
+        if constexpr (MODE == M_CHAN) { b[k] = p.b[ci]; if (rs) rr[k].load(rs + (size_t)ci * p.HW); }
+    }
+    if (MODE == M_RMS && rs) {
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int c = g + G * k, ci = c < p.C ? c : 0;
+            V8<T> a; a.load(rs + (size_t)ci * p.HW);
+            float h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = xr[k].get(j) + a.get(j);
+            xr[k].set(h);
+            if (ok && c < p.C) xr[k].store((T*)p.h + base + (size_t)c * p.HW);
+        }
+    }
+    float mu[8], acc[8];
+    unsigned am[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { mu[j] = 0.f; acc[j] = 0.f; am[j] = 0; }
+    if constexpr (MODE == M_CHAN) {
+#pragma unroll
+        for (int k = 0; k < CPT; ++k)
+            if (g + G * k < p.C)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[j] += xr[k].get(j);
+        tile_reduce<LPX, false>(acc, red[wave]);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = pl * 8 + j;
+            mu[j] = ((red[0][i] + red[1][i]) + (red[2][i] + red[3][i])) / (float)p.C;
+            acc[j] = 0.f;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < CPT; ++k)
+        if (g + G * k < p.C)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = xr[k].get(j) - mu[j];
+                acc[j] += d * d;
+                if (FMT != Q_NONE) am[j] = umax(am[j], abs_bits(MODE == M_RMS && p.q_of_y ? d * w[k] : d));
+            }
+    tile_reduce<LPX, false>(acc, red[wave]);
+    if (FMT != Q_NONE) tile_reduce<LPX, true>(am, redm[wave]);
+    __syncthreads();
+    if (tid < TP) {
+        const float ss = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+        const float r = rsqrtf(ss / (float)(MODE == M_RMS ? p.C : p.C - 1) + p.eps);
+        st_r[tid] = r;
+        if (p.rstd && sok) p.rstd[stok] = r;
+        if (FMT != Q_NONE) {
+            // max|d| r = max|d r|: a rounded product is monotone (with q_of_y the weight comes between, and q8_pack8 clamps)
+            const unsigned m = umax(umax(redm[0][tid], redm[1][tid]), umax(redm[2][tid], redm[3][tid]));
+            const unsigned code = q8_code<F>(abs_bits(__uint_as_float(m) * r));
+            st_inv[tid] = q8_inv_scale(code);
+            if (sok) p.qe[stok] = (u8_t)code;
+        }
+    }
+    __syncthreads();
+    float r[8], inv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { r[j] = st_r[pl * 8 + j]; if (FMT != Q_NONE) inv[j] = st_inv[pl * 8 + j]; am[j] = 0; }
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int c = g + G * k;
+        if (c >= p.C) continue;
+        const size_t at = base + (size_t)c * p.HW;
+        float xh[8], o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            xh[j] = (xr[k].get(j) - mu[j]) * r[j];
+            o[j] = MODE == M_RMS ? xh[j] * w[k] : fmaf(w[k], xh[j], b[k]);
+        }
+        if constexpr (FMT != Q_NONE) {
+            u32x2_t q;
+            if (MODE == M_CHAN && p.relu) q = q8_pack8_masked<F>(xh, inv, o, w[k], b[k]);
+            else {
+                float t[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) t[j] = (MODE == M_RMS && p.q_of_y ? o[j] : xh[j]) * inv[j];
+                q = q8_pack8<F, MODE == M_RMS>(t);
+            }
+            if (ok) *(u32x2_a1*)(p.q + at) = q;
+        }
+        if constexpr (MODE == M_CHAN) {
+            if (p.relu)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = relu_nan(o[j]);
+            if (rs) {                    // both terms rounded to the storage type first, as norm and add one after the other
+                V8<T> t; t.set(o);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { o[j] = t.get(j) + rr[k].get(j); if (FMT != Q_NONE) am[j] = umax(am[j], abs_bits(o[j])); }
+                if (p.q2) {              // the sum replaces x: kept in float32 precision by its two terms until the exponent is known
+                    xr[k] = t;
+                }
+            }
+        }
+        if (p.y && ok) { V8<T> t; t.set(o); t.store((T*)p.y + at); }
+    }
+    if constexpr (MODE == M_CHAN && FMT != Q_NONE) {
+        if (!p.q2) return;
+        tile_reduce<LPX, true>(am, redm[wave]);          // (its readers of the first maximum are behind two barriers)
+        __syncthreads();
+        if (tid < TP) {
+            const unsigned code = q8_code<F>(umax(umax(redm[0][tid], redm[1][tid]), umax(redm[2][tid], redm[3][tid])));
+            st_inv[tid] = q8_inv_scale(code);
+            if (sok) p.qe2[stok] = (u8_t)code;
+        }
+        __syncthreads();
+        if (!ok) return;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) inv[j] = st_inv[pl * 8 + j];
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int c = g + G * k;
+            if (c >= p.C) continue;
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = (xr[k].get(j) + rr[k].get(j)) * inv[j];
+            *(u32x2_a1*)(p.q2 + base + (size_t)c * p.HW) = q8_pack8<F, false>(t);
+        }
+    }
+}
+
+// Rows of eight channels and more (root-mean-square norm): eight channels per lane, L lanes and K groups per lane for a row.
+template <typename T, int FMT, int L, int K>
+__global__ __launch_bounds__(256) void rms_fwd_rows_kernel(const NormFwd p, int N) {
+    constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;
+    const int l = threadIdx.x % L;
+    const long long row0 = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const bool ok = row0 < N;
+    const size_t base = (size_t)(ok ? row0 : N - 1) * p.C;
+    const unsigned C = p.C;
+    V8<T> xr[K], rr[K];
+    V8<float> w[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned c = umin((unsigned)(l + L * k) * 8, C - 8);
+        xr[k].load((const T*)p.x + base + c);
+        if (p.resid) rr[k].load((const T*)p.resid + base + c);
+        w[k].load(p.w + c);
+    }
+    float ss = 0.f;
+    unsigned am = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned cn = (unsigned)(l + L * k) * 8, c = umin(cn, C - 8);
+        if (p.resid) {
+            float h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = xr[k].get(j) + rr[k].get(j);
+            xr[k].set(h);
+            if (ok && cn < C) xr[k].store((T*)p.h + base + c);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // a group past the end was moved back: its first values belong to the group before it
+            const float v = c + j >= cn ? xr[k].get(j) : 0.f;
+            ss += v * v;
+            if (FMT != Q_NONE) am = umax(am, abs_bits(p.q_of_y ? v * w[k].get(j) : v));
+        }
+    }
+    ss = row_sum<L>(ss);
+    const float r = rsqrtf(ss / (float)C + p.eps);
+    float inv = 0.f;
+    if constexpr (FMT != Q_NONE) {
+        const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(am)) * r));
+        inv = q8_inv_scale(code);
+        if (ok && l == 0) p.qe[row0] = (u8_t)code;
+    }
+    if (!ok) return;
+    if (p.rstd && l == 0) p.rstd[row0] = r;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned cn = (unsigned)(l + L * k) * 8;
+        if (cn >= C) continue;
+        const size_t at = base + umin(cn, C - 8);
+        float xh[8], o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { xh[j] = xr[k].get(j) * r; o[j] = xh[j] * w[k].get(j); }
+        if constexpr (FMT != Q_NONE) {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = (p.q_of_y ? o[j] : xh[j]) * inv;
+            *(u32x2_a1*)(p.q + at) = q8_pack8<F, true>(t);
+        }
+        if (p.y) { V8<T> t; t.set(o); t.store((T*)p.y + at); }
     }
 }
 
@@ -195,6 +413,223 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
     }
 }
 
+// Planes: as norm8_fwd_tile_kernel.  A workgroup takes `pit` tiles of one image in turn and keeps the sums of its channels in
+// registers: part[workgroup][0..2][c] as norm8_param_kernel.
+template <typename T, int MODE, int SRC, int LPX, int CPT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
+    constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
+    __shared__ float red[2][4][TP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
+    const unsigned per = (p.tiles + pit - 1) / pit;                  // workgroups per image
+    const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / per, t0 = (bid - n * per) * pit;
+    const unsigned octs = ((unsigned)p.HW + 7) >> 3;
+    float w[CPT], b[MODE == M_CHAN ? CPT : 1], pg[CPT], pb[MODE == M_CHAN ? CPT : 1], pd[MODE == M_CHAN ? CPT : 1];
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int c = g + G * k, ci = c < p.C ? c : 0;
+        w[k] = p.w[ci]; pg[k] = 0.f;
+        if constexpr (MODE == M_CHAN) { b[k] = p.b[ci]; pb[k] = 0.f; pd[k] = 0.f; }
+    }
+    for (unsigned it = 0; it < pit && t0 + it < p.tiles; ++it) {
+        const unsigned oct = (t0 + it) * LPX + pl;
+        const bool ok = oct < octs;
+        const unsigned hw0 = umin(ok ? oct * 8 : 0u, (unsigned)p.HW - 8);
+        const int dup = ok ? (int)(oct * 8 - hw0) : 8;               // values that another lane adds to the channels' sums
+        const size_t base = (size_t)n * p.C * p.HW + hw0, tok = (size_t)n * p.HW + hw0;
+        V8<T> dy[CPT], hr[SRC == SRC_T ? CPT : 1], ds[MODE == M_RMS ? CPT : 1];
+        u32x2_t q[SRC == SRC_T ? 1 : CPT];
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int c = g + G * k;
+            const size_t at = base + (size_t)(c < p.C ? c : 0) * p.HW;
+            if constexpr (SRC == SRC_T) hr[k].load((const T*)p.h + at); else q[k] = *(const u32x2_a1*)(p.q + at);
+            dy[k].load((const T*)p.dy + at);
+            if constexpr (MODE == M_RMS) if (p.dstream) ds[k].load((const T*)p.dstream + at);
+        }
+        V8<float> r; r.load(p.rstd + tok);
+        float sc[8];
+        if constexpr (SRC == SRC_T) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[j] = r.get(j);
+        } else {
+            const u32x2_t e = *(const u32x2_a1*)(p.qe + tok);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc[j] = q8_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
+        }
+        auto values = [&](int k, float* xh) {
+            if constexpr (SRC == SRC_T) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * sc[j];
+            } else {
+                q8_unpack8<SRC>(q[k], xh);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xh[j] *= sc[j];
+            }
+        };
+        float s1[8], s2[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s1[j] = 0.f; s2[j] = 0.f; }
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            if (g + G * k >= p.C) continue;
+            float xh[8];
+            values(k, xh);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float d = dy[k].get(j);
+                if (MODE == M_CHAN && p.relu && !(fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]) > 0.f)) d = 0.f;
+                const float dk = j >= dup ? d : 0.f;
+                pg[k] += dk * xh[j];
+                if constexpr (MODE == M_CHAN) pb[k] += dk;
+                d *= w[k];
+                if (MODE == M_CHAN) s1[j] += d;
+                s2[j] += d * xh[j];
+            }
+        }
+        if (it > 0) __syncthreads();                                 // the readers of the previous tile's sums are done
+        tile_reduce<LPX, false>(s2, red[1][wave]);
+        if (MODE == M_CHAN) tile_reduce<LPX, false>(s1, red[0][wave]);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = pl * 8 + j;
+            s2[j] = ((red[1][0][i] + red[1][1][i]) + (red[1][2][i] + red[1][3][i])) / (float)(MODE == M_RMS ? p.C : p.C - 1);
+            if (MODE == M_CHAN) s1[j] = ((red[0][0][i] + red[0][1][i]) + (red[0][2][i] + red[0][3][i])) / (float)p.C;
+        }
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int c = g + G * k;
+            if (c >= p.C) continue;
+            float xh[8], o[8];
+            values(k, xh);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float d = dy[k].get(j);
+                if (MODE == M_CHAN && p.relu && !(fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]) > 0.f)) d = 0.f;
+                d = d * w[k] - xh[j] * s2[j];
+                if (MODE == M_CHAN) d -= s1[j];
+                o[j] = d * r.get(j);
+                if constexpr (MODE == M_RMS) if (p.dstream) o[j] += ds[k].get(j);
+            }
+            V8<T> t; t.set(o);
+            if (ok) t.store((T*)p.dx + base + (size_t)c * p.HW);
+            if constexpr (MODE == M_CHAN)
+                if (p.db)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) pd[k] += j >= dup ? t.get(j) : 0.f;      // what the tensor holds
+        }
+    }
+    float* part = p.part + (size_t)bid * (MODE == M_RMS ? 1 : 2 + p.db) * p.C;
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int c = g + G * k;
+#pragma unroll
+        for (int o = LPX >> 1; o > 0; o >>= 1) {
+            pg[k] += __shfl_xor(pg[k], o, 64);
+            if constexpr (MODE == M_CHAN) { pb[k] += __shfl_xor(pb[k], o, 64); pd[k] += __shfl_xor(pd[k], o, 64); }
+        }
+        if (pl == 0 && c < p.C) {
+            part[c] = pg[k];
+            if constexpr (MODE == M_CHAN) { part[p.C + c] = pb[k]; if (p.db) part[2 * p.C + c] = pd[k]; }
+        }
+    }
+}
+
+// Rows: a workgroup takes every gridDim.x-th group of 256 / L rows and keeps the sums of its channels in registers.
+template <typename T, int SRC, int L, int K>
+__global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int N) {
+    constexpr int R = 256 / L;
+    __shared__ float red[R][L][8];
+    const int l = threadIdx.x % L, rg = threadIdx.x / L;
+    const unsigned C = p.C;
+    V8<float> w[K];
+    float pg[K][8];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        w[k].load(p.w + umin((unsigned)(l + L * k) * 8, C - 8));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pg[k][j] = 0.f;
+    }
+    for (long long r0 = (long long)blockIdx.x * R; r0 < N; r0 += (long long)gridDim.x * R) {
+        const bool ok = r0 + rg < N;
+        const long long row = ok ? r0 + rg : N - 1;
+        const size_t base = (size_t)row * C;
+        V8<T> dy[K], hr[SRC == SRC_T ? K : 1], ds[K];
+        u32x2_t q[SRC == SRC_T ? 1 : K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const size_t at = base + umin((unsigned)(l + L * k) * 8, C - 8);
+            if constexpr (SRC == SRC_T) hr[k].load((const T*)p.h + at); else q[k] = *(const u32x2_a1*)(p.q + at);
+            dy[k].load((const T*)p.dy + at);
+            if (p.dstream) ds[k].load((const T*)p.dstream + at);
+        }
+        const float r = p.rstd[row];
+        float sc = r;
+        if constexpr (SRC != SRC_T) sc = q8_scale(p.qe[row]);
+        auto values = [&](int k, float* xh) {
+            if constexpr (SRC == SRC_T) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * sc;
+            } else {
+                q8_unpack8<SRC>(q[k], xh);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xh[j] *= sc;
+            }
+        };
+        float s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const unsigned cn = (unsigned)(l + L * k) * 8, c = umin(cn, C - 8);
+            float xh[8];
+            values(k, xh);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = c + j >= cn ? dy[k].get(j) * xh[j] : 0.f;
+                pg[k][j] += ok ? d : 0.f;
+                s2 += d * w[k].get(j);
+            }
+        }
+        s2 = row_sum<L>(s2) / (float)C;
+        if (!ok) continue;               // (only the last round has rows that are not there, and none of its lanes waits again)
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const unsigned cn = (unsigned)(l + L * k) * 8;
+            if (cn >= C) continue;
+            float xh[8], o[8];
+            values(k, xh);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                o[j] = (dy[k].get(j) * w[k].get(j) - xh[j] * s2) * r;
+                if (p.dstream) o[j] += ds[k].get(j);
+            }
+            V8<T> t; t.set(o);
+            t.store((T*)p.dx + base + umin(cn, C - 8));
+        }
+    }
+    float* part = p.part + (size_t)blockIdx.x * C;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const unsigned cn = (unsigned)(l + L * k) * 8, c = umin(cn, C - 8);
+        if (R > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) red[rg][l][j] = pg[k][j];
+            __syncthreads();
+            if (rg != 0) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float s = 0.f;
+                for (int i = 0; i < R; ++i) s += red[i][l][j];
+                pg[k][j] = s;
+            }
+        }
+        if (cn < C)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j >= cn) part[c + j] = pg[k][j];
+    }
+}
+
 // column sums of part[rows][nr * C] into up to three vectors, each written or added to: 64 columns x 16 row lanes, fixed order
 __global__ __launch_bounds__(1024) void norm8_colsum_kernel(const float* __restrict__ part, float* __restrict__ d0, float* __restrict__ d1,
                                                             float* __restrict__ d2, int C, int rows, int nr, int acc, int acc2) {
@@ -231,9 +666,57 @@ int norm8_nsplit(int N, int C, int HW) {                             // ~1024 wo
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s);
 }
+// tiles per workgroup of the backward plane kernel: ~2048 workgroups, so that few rows of channel sums are written
+unsigned norm8_pit(const TileCfg& t, long long N) {
+    unsigned pit = (unsigned)(t.blocks / 2048);
+    return pit < 1 ? 1 : (pit > t.tiles ? t.tiles : pit);
+}
+// channels per thread that the forward / backward plane kernels keep in registers
+template <typename T> constexpr int tile_most(bool bwd) { return sizeof(T) == 2 ? 8 : (bwd ? 4 : 8); }
+// rows of channel sums that the backward pass writes
+template <typename T>
+size_t norm8_rows(int mode, int N, int C, int HW) {
+    if (HW >= 8) {
+        const TileCfg t = tile_pick(N, C, HW, tile_most<T>(true));
+        if (t.lpx) return (size_t)cdiv((int)t.tiles, (int)norm8_pit(t, N)) * N;
+    }
+    if (mode == M_RMS && HW == 1 && C >= 8) {
+        const RowCfg r = row_pick(N, C);
+        if (r.l) { const int g = cdiv(N, 256 / r.l); return (size_t)(g < 1024 ? g : 1024); }
+    }
+    return (size_t)norm8_nsplit(N, C, HW);
+}
+
+#define NORM8_TILE(T, t, F)                                                                                               \
+    do {                                                                                                                  \
+        if ((t).lpx == 8) { NORM8_CPT(T, 8, t, F); } else if ((t).lpx == 4) { NORM8_CPT(T, 4, t, F); }                    \
+        else if ((t).lpx == 2) { NORM8_CPT(T, 2, t, F); } else { NORM8_CPT(T, 1, t, F); }                                 \
+    } while (0)
+#define NORM8_CPT(T, LPX, t, F)                                                                                           \
+    if ((t).cpt <= 1) F(LPX, 1); else if ((t).cpt <= 2) F(LPX, 2); else if ((t).cpt <= 4) F(LPX, 4); else F(LPX, 8)
 
 template <typename T, int MODE, int FMT>
 int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
+    if (p.HW >= 8) {
+        const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>(false));
+        if (t.lpx) {
+            if (t.blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
+            p.tiles = t.tiles;
+#define FWD(LPX, CPT) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, LPX, CPT>), dim3((unsigned)t.blocks), dim3(256), 0, st, p, (unsigned)t.blocks)
+            NORM8_TILE(T, t, FWD);
+#undef FWD
+            return hific_launch_status();
+        }
+    }
+    if constexpr (MODE == M_RMS) {
+        RowCfg r;
+        if (p.HW == 1 && p.C >= 8 && (r = row_pick(N, p.C)).l) {
+#define ROWS(L, K) hipLaunchKernelGGL((rms_fwd_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, 256 / L)), dim3(256), 0, st, p, N)
+            ROW_DISPATCH(r, ROWS)
+#undef ROWS
+            return hific_launch_status();
+        }
+    }
     const int px = norm8_px(p.HW);
     const long long blocks = cdivl(p.HW, px) * N;
     if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
@@ -247,22 +730,48 @@ int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
 
 template <typename T, int MODE, int SRC>
 int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc, int acc2, size_t ws_bytes, hipStream_t st) {
-    const int px = norm8_px(p.HW), nr = MODE == M_RMS ? 1 : 2 + p.db;
-    const long long blocks = cdivl(p.HW, px) * N;
-    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-    p.tiles = (unsigned)cdivl(p.HW, px);
-    p.tokens = (long long)N * p.HW;
-    p.nsplit = norm8_nsplit(N, p.C, p.HW);
-    if ((size_t)p.nsplit * nr * p.C * sizeof(float) > ws_bytes) return HIFIC_ERR_WS;
-    const dim3 grid((unsigned)blocks), pgrid(cdiv(p.C, 256 / px), p.nsplit);
-#define BWD(PX)                                                                                             \
-    do {                                                                                                    \
-        hipLaunchKernelGGL((norm8_bwd_kernel<T, MODE, SRC, PX>), grid, dim3(256), 0, st, p);               \
-        hipLaunchKernelGGL((norm8_param_kernel<T, MODE, SRC, PX>), pgrid, dim3(256), 0, st, p);            \
-    } while (0)
-    if (px == 1) BWD(1); else if (px == 16) BWD(16); else BWD(64);
+    const int nr = MODE == M_RMS ? 1 : 2 + p.db;
+    const size_t rows = norm8_rows<T>(MODE, N, p.C, p.HW);
+    if (rows * nr * p.C * sizeof(float) > ws_bytes) return HIFIC_ERR_WS;
+    TileCfg t{0, 0, 0, 0};
+    RowCfg r{0, 0};
+    if (p.HW >= 8) t = tile_pick(N, p.C, p.HW, tile_most<T>(true));
+    else if (MODE == M_RMS && p.HW == 1 && p.C >= 8) r = row_pick(N, p.C);
+    if (rows > 0x7fffffffull) return HIFIC_ERR_UNSUPPORTED;
+    if (t.lpx) {
+        p.tiles = t.tiles;
+        const unsigned pit = norm8_pit(t, N);
+#define BWD(LPX, CPT) hipLaunchKernelGGL((norm8_bwd_tile_kernel<T, MODE, SRC, LPX, CPT>), dim3((unsigned)rows), dim3(256), 0, st, p, (unsigned)rows, pit)
+        if constexpr (tile_most<T>(true) == 8) NORM8_TILE(T, t, BWD);
+        else {
+#undef NORM8_CPT
+#define NORM8_CPT(T, LPX, t, F) if ((t).cpt <= 1) F(LPX, 1); else if ((t).cpt <= 2) F(LPX, 2); else F(LPX, 4)
+            NORM8_TILE(T, t, BWD);
+        }
 #undef BWD
-    hipLaunchKernelGGL(norm8_colsum_kernel, dim3(cdiv(nr * p.C, 64)), dim3(1024), 0, st, p.part, d0, d1, d2, p.C, p.nsplit, nr, acc, acc2);
+    } else if (r.l) {
+        if constexpr (MODE == M_RMS) {
+#define ROWS(L, K) hipLaunchKernelGGL((rms_bwd_rows_kernel<T, SRC, L, K>), dim3((unsigned)rows), dim3(256), 0, st, p, N)
+            ROW_DISPATCH(r, ROWS)
+#undef ROWS
+        }
+    } else {
+        const int px = norm8_px(p.HW);
+        const long long blocks = cdivl(p.HW, px) * N;
+        if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
+        p.tiles = (unsigned)cdivl(p.HW, px);
+        p.tokens = (long long)N * p.HW;
+        p.nsplit = (int)rows;
+        const dim3 grid((unsigned)blocks), pgrid(cdiv(p.C, 256 / px), p.nsplit);
+#define BWD(PX)                                                                                                 \
+        do {                                                                                                    \
+            hipLaunchKernelGGL((norm8_bwd_kernel<T, MODE, SRC, PX>), grid, dim3(256), 0, st, p);               \
+            hipLaunchKernelGGL((norm8_param_kernel<T, MODE, SRC, PX>), pgrid, dim3(256), 0, st, p);            \
+        } while (0)
+        if (px == 1) BWD(1); else if (px == 16) BWD(16); else BWD(64);
+#undef BWD
+    }
+    hipLaunchKernelGGL(norm8_colsum_kernel, dim3(cdiv(nr * p.C, 64)), dim3(1024), 0, st, p.part, d0, d1, d2, p.C, (int)rows, nr, acc, acc2);
     return hific_launch_status();
 }
 }  // namespace
@@ -283,7 +792,13 @@ int hific_rms_norm_fwd(const void* x, const void* resid, const float* w, void* y
 
 size_t hific_norm8_bwd_ws_bytes(int N, int C, int HW) {
     if (N <= 0 || C <= 0 || HW <= 0) return 0;
-    return (size_t)norm8_nsplit(N, C, HW) * 3 * C * sizeof(float);
+    size_t rows = 0;
+    for (int mode : {M_RMS, M_CHAN}) {
+        const size_t a = norm8_rows<float>(mode, N, C, HW), b = norm8_rows<bf16_t>(mode, N, C, HW);
+        rows = a > rows ? a : rows;
+        rows = b > rows ? b : rows;
+    }
+    return rows * 3 * C * sizeof(float);
 }
 
 int hific_rms_norm_bwd(const void* h, const void* q, const void* qe, int fmt, const float* rstd, const void* dy, const void* dstream,
