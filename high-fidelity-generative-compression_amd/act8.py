@@ -7,22 +7,17 @@ keep what their backward pass needs in it (1 byte per element in the place of a 
 and `conv2d_weight_grad8` / `conv_transpose2d_weight_grad8` contract one.  The functions are part of `hific_amd.ops`.
 """
 import contextlib
+import functools
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from . import lib
-from .lib import call, ptr, stream, require_gpu
+from . import lib, ops
+from .lib import ptr, stream, require_gpu
 
 FORMATS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
-_here = contextlib.nullcontext()
-
-
-def _on(t):
-    """Context in which launches go to the device of `t` (and to that device's current stream)."""
-    return _here if t.device.index == lib._cur_device() else torch.cuda.device(t.device)
+_INF = float("inf")
 
 
 def _fmt(fmt):
@@ -33,57 +28,78 @@ def _fmt(fmt):
 
 def _nchw(x, name="x"):
     """(N, C, positions) of an activation [N, C, ...]."""
-    if x.dim() < 2 or x.shape[1] < 1:
+    d = x.dim()
+    if d < 2 or x.size(1) < 1:
         raise lib.HificError(f"{name} must be [N, C, ...] with at least one channel, got {tuple(x.shape)}")
     hw = 1
-    for d in x.shape[2:]:
-        hw *= d
-    return x.shape[0], x.shape[1], hw
+    for i in range(2, d):
+        hw *= x.size(i)
+    return x.size(0), x.size(1), hw
 
 
 def _tokens(x):
     return x.shape[:1] + x.shape[2:]
 
 
-def _act(x):
-    require_gpu_any(x)
-    lib.dtype_code(x)                                   # float32 or bfloat16
-    return c16(x)
-
-
-def require_gpu_any(*tensors):
-    """require_gpu without the contiguity rule (strided tensors are copied), and all on one device."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            require_gpu(t)
-        if dev is not None and t.device != dev:
-            raise lib.HificError(f"tensors on {dev} and {t.device}")
-        dev = t.device
+def _one_device(first, *rest):
+    """All on the GPU, and on one (strided tensors are copied later: no contiguity rule)."""
+    if not first.is_cuda:
+        require_gpu(first)
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            if not t.is_cuda:
+                require_gpu(t)
+            raise lib.HificError(f"tensors on {first.device} and {t.device}")
 
 
 def c16(t):
-    """Contiguous and 16-byte aligned (the wide kernels' accesses): a strided or oddly placed view is copied."""
-    t = t.contiguous()
+    """Contiguous and 16-byte aligned: a strided or oddly placed view is copied."""
+    if not t.is_contiguous():
+        return t.contiguous()
     return t if (t.data_ptr() & 15) == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _param(w, C, name):
-    if w.dtype != torch.float32 or w.numel() != C or not w.is_contiguous():
+    if w.dtype is not torch.float32 or w.numel() != C or not w.is_contiguous():
         raise lib.HificError(f"{name} must be a contiguous float32 tensor of {C} values, got {w.dtype} {tuple(w.shape)}")
 
 
 def _like(t, x, name):
-    if t.shape != x.shape or t.dtype != x.dtype:
+    if t.dtype is not x.dtype or t.shape != x.shape:
         raise lib.HificError(f"{name} must be {x.dtype} {tuple(x.shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _eps(eps):
-    if not 0.0 < eps < float("inf"):
+    if not 0.0 < eps < _INF:
         raise lib.HificError(f"eps must be positive and finite, got {eps}")
     return float(eps)
+
+
+def _launch(name, t, *args):
+    """Entry point `name` on the device of `t` and its current stream (the last argument)."""
+    fn = getattr(lib._lib, name)
+    if t.get_device() == lib._cur_device():
+        rc = fn(*args, stream())
+    else:
+        with _on(t):
+            rc = fn(*args, stream())
+    if rc != 0:
+        raise lib.HificError(f"{name} failed: {lib._ERR.get(rc, rc)} (rc={rc})")
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(t):
+    """Context in which launches (and the stream's workspace) belong to the device of `t`."""
+    return _here if t.get_device() == lib._cur_device() else torch.cuda.device(t.device)
+
+
+def _first_order(*grads):
+    # grad mode is on in a backward pass with create_graph=True only
+    if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
+        raise lib.HificError("the 8-bit activation operators have no second derivative")
 
 
 class Act8:
@@ -99,11 +115,18 @@ class Act8:
             raise lib.HificError(f"Act8: e must be {tuple(_tokens(q))} for q {tuple(q.shape)}, got {tuple(e.shape)}")
         if (gamma is None) != (beta is None) or (relu and gamma is None):
             raise lib.HificError("Act8: gamma and beta come together, and relu with them")
-        require_gpu_any(q, e, gamma, beta)
+        _one_device(q, e, gamma, beta)
         for t, name in ((gamma, "gamma"), (beta, "beta")):
             if t is not None:
                 _param(t, C, name)
         self.q, self.e, self.gamma, self.beta, self.relu = c16(q), c16(e), gamma, beta, bool(relu)
+
+    @classmethod
+    def _of(cls, q, e, gamma=None, beta=None, relu=False):
+        """Without the checks: tensors that were just made."""
+        a = object.__new__(cls)
+        a.q, a.e, a.gamma, a.beta, a.relu = q, e, gamma, beta, relu
+        return a
 
     @property
     def fmt(self):
@@ -123,19 +146,20 @@ class Act8:
 
 
 def _new8(x, dt):
-    return torch.empty(x.shape, dtype=dt, device=x.device), torch.empty(_tokens(x), dtype=torch.uint8, device=x.device)
+    return torch.empty_like(x, dtype=dt), torch.empty(_tokens(x), dtype=torch.uint8, device=x.device)
 
 
 def checkpoint8(x, fmt="int8"):
     """x (float32 or bfloat16, [N, C, ...]) -> Act8.  Carries no gradient: it is what a backward pass keeps of x."""
     code, dt = _fmt(fmt)
     N, C, HW = _nchw(x)
-    x = _act(x.detach())
+    _one_device(x)
+    x = c16(x.detach())
+    cd = lib.dtype_code(x)
     q, e = _new8(x, dt)
-    if x.numel():
-        with _on(x):
-            call("hific_act8_pack", ptr(x), ptr(q), ptr(e), code, N, C, HW, lib.dtype_code(x), stream())
-    return Act8(q, e)
+    if N and HW:
+        _launch("hific_act8_pack", x, x.data_ptr(), q.data_ptr(), e.data_ptr(), code, N, C, HW, cd)
+    return Act8._of(q, e)
 
 
 def restore8(a, dtype=torch.bfloat16):
@@ -148,145 +172,141 @@ def restore8(a, dtype=torch.bfloat16):
 
 
 def _restore(q, e, gamma, beta, relu, dtype):
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    if out.numel():
-        N, C, HW = _nchw(q)
-        with _on(q):
-            call("hific_act8_restore", ptr(q), ptr(e), _CODE[q.dtype], ptr(gamma), ptr(beta), int(relu), ptr(out), N, C, HW,
-                 lib.dtype_code(out), stream())
+    out = torch.empty_like(q, dtype=dtype)
+    N, C, HW = _nchw(q)
+    if N and HW:
+        _launch("hific_act8_restore", q, q.data_ptr(), e.data_ptr(), _CODE[q.dtype], ptr(gamma), ptr(beta), int(relu), out.data_ptr(),
+                N, C, HW, lib.HIFIC_F32 if dtype is torch.float32 else lib.HIFIC_BF16)
     return out
 
 
 # ---- root-mean-square norm ---------------------------------------------------------------------------------------------
-def _rms_fwd(x, weight, resid, eps, code, dt, want_y, want_rstd, q_of_y):
-    """-> y, h, rstd, q, e (None where not asked for; h is x without a residual)."""
-    N, C, HW = _nchw(x)
+def _rms_fwd(x, weight, resid, eps, geom, cd, code, dt, want_y, want_rstd):
+    """-> y, h, rstd, q, e (None where not asked for; q holds y where y is not asked for, else the normalised values)."""
+    N, C, HW = geom
     y = torch.empty_like(x) if want_y else None
     h = torch.empty_like(x) if resid is not None else None
     rstd = torch.empty(_tokens(x), dtype=torch.float32, device=x.device) if want_rstd else None
     q, e = _new8(x, dt) if dt is not None else (None, None)
-    if x.numel():
-        with _on(x):
-            call("hific_rms_norm_fwd", ptr(x), ptr(resid), ptr(weight), ptr(y), ptr(h), ptr(rstd), ptr(q), ptr(e), code,
-                 int(q_of_y), N, C, HW, eps, lib.dtype_code(x), stream())
+    if N and HW:
+        _launch("hific_rms_norm_fwd", x, x.data_ptr(), ptr(resid), weight.data_ptr(), ptr(y), ptr(h), ptr(rstd), ptr(q), ptr(e), code,
+                0 if want_y else 1, N, C, HW, eps, cd)
     return y, h, rstd, q, e
+
+
+@functools.lru_cache(maxsize=1024)
+def _bwd_ws_bytes(N, C, HW):
+    return int(lib.raw("hific_norm8_bwd_ws_bytes")(N, C, HW))
 
 
 def _bwd_ws(N, C, HW, device):
     # its own allocation per call, not the stream's workspace: two captured graphs that replay on two streams share nothing
-    n = int(lib.raw("hific_norm8_bwd_ws_bytes")(N, C, HW))
+    n = _bwd_ws_bytes(N, C, HW)
     return torch.empty(n, dtype=torch.uint8, device=device), n
 
 
-def _rms_bwd(h, q, e, rstd, dy, dstream, weight, dw, acc):
-    N, C, HW = _nchw(dy)
-    dx = torch.empty_like(dy)
-    if dy.numel():
-        ws, n = _bwd_ws(N, C, HW, dy.device)
-        call("hific_rms_norm_bwd", ptr(h), ptr(q), ptr(e), 0 if q is None else _CODE[q.dtype], ptr(rstd), ptr(dy), ptr(dstream),
-             ptr(weight), ptr(dx), ptr(dw), acc, N, C, HW, lib.dtype_code(dy), ptr(ws), n, stream())
-    elif not acc:
-        dw.zero_()
-    return dx
-
-
 class RmsNormFn(Function):
-    """y = weight * h * rsqrt(mean_c h^2 + eps), h = x + resid.  Keeps h (or x), or with `fmt` its normalised form in 8 bits."""
+    """y = weight * h * rsqrt(mean_c h^2 + eps), h = x + resid.  Keeps h (or x), or with a format its normalised form in 8 bits."""
 
     @staticmethod
-    def forward(ctx, x, weight, resid, eps, fmt):
-        from . import ops
-        code, dt = _fmt(fmt) if fmt is not None else (0, None)
-        y, h, rstd, q, e = _rms_fwd(x, weight, resid, eps, code, dt, True, True, False)
-        ctx.slot = ops._slot(weight)
-        ctx.has_resid, ctx.kept8 = resid is not None, fmt is not None
+    def forward(ctx, x, weight, resid, eps, geom, cd, code, dt):
+        y, h, rstd, q, e = _rms_fwd(x, weight, resid, eps, geom, cd, code, dt, True, True)
+        ctx.geom, ctx.cd, ctx.code, ctx.slot = geom, cd, code, ops._slot(weight)
+        ctx.has_resid = resid is not None
         ctx.set_materialize_grads(False)
-        if fmt is not None:
+        if dt is not None:
             ctx.save_for_backward(q, e, rstd, weight)
         else:
-            ctx.save_for_backward(x if resid is None else h, rstd, weight)
-        return y if resid is None else (y, h)
+            ctx.save_for_backward(x if h is None else h, None, rstd, weight)
+        return y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dstream=None):
-        from . import ops
-        if ctx.kept8:
-            q, e, rstd, weight = ctx.saved_tensors
-            h = None
-        else:
-            h, rstd, weight = ctx.saved_tensors
-            q = e = None
-        want_w = ctx.needs_input_grad[1]
+        _first_order(dy, dstream)
+        kept, e, rstd, weight = ctx.saved_tensors
+        none = (None,) * 5
         if dy is None:                                   # only the stream was used
-            return dstream, None, (dstream if ctx.has_resid else None), None, None
+            return (dstream, None, dstream if ctx.has_resid else None) + none
         dy = c16(dy)
-        dstream = None if dstream is None else c16(dstream)
-        with _on(dy):
-            if want_w:
-                dwt, acc, dw = ops._grad_target(ctx.slot, weight)
-            else:
-                dwt, acc, dw = torch.empty_like(weight), 0, None
-            dx = _rms_bwd(h, q, e, rstd, dy, dstream, weight, dwt, acc)
-            if want_w:
-                ops._written(ctx.slot)
-        return dx, dw, (dx if ctx.has_resid else None), None, None
+        if dstream is not None:
+            dstream = c16(dstream)
+        want_w = ctx.needs_input_grad[1]
+        dwt, acc, dw = ops._grad_target(ctx.slot, weight) if want_w else (torch.empty_like(weight), 0, None)
+        dx = torch.empty_like(dy)
+        N, C, HW = ctx.geom
+        if N and HW:
+            ws, n = _bwd_ws(N, C, HW, dy.device)
+            h, q = (kept.data_ptr(), None) if e is None else (None, kept.data_ptr())
+            _launch("hific_rms_norm_bwd", dy, h, q, ptr(e), ctx.code, rstd.data_ptr(), dy.data_ptr(), ptr(dstream), weight.data_ptr(),
+                    dx.data_ptr(), dwt.data_ptr(), acc, N, C, HW, ctx.cd, ws.data_ptr(), n)
+        elif not acc:
+            dwt.zero_()
+        if want_w:
+            ops._written(ctx.slot)
+        return (dx, dw, dx if ctx.has_resid else None) + none
 
 
-def _rms_args(x, weight, resid, eps):
-    _, C, _ = _nchw(x)
-    require_gpu_any(x, weight, resid)
-    _param(weight, C, "weight")
+def _rms_args(x, weight, resid):
+    """-> x, resid (contiguous, aligned), (N, C, positions), type code."""
+    geom = _nchw(x)
+    _one_device(x, weight, resid)
+    _param(weight, geom[1], "weight")
     if resid is not None:
         _like(resid, x, "resid")
-        resid = _act(resid)
-    return _act(x), resid, _eps(eps)
+        resid = c16(resid)
+    return c16(x), resid, geom, lib.dtype_code(x)
+
+
+def _needs_grad(x, weight, resid):
+    return torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (resid is not None and resid.requires_grad))
 
 
 def rms_norm(x, weight, resid=None, eps=1e-6, fmt=None):
     """weight * h / sqrt(mean_c h^2 + eps) over dim 1 of x [N, C, ...] (float32 or bfloat16; weight float32, C values).
     With `resid` (like x): h = x + resid rounded to x's type, and (y, h) is returned - h is the new residual stream, and the norm
     and its backward pass see what it holds.  `fmt` ("int8" | "e4m3"): the backward pass keeps h in 8 bits, normalised."""
-    x, resid, eps = _rms_args(x, weight, resid, eps)
-    if fmt is not None:
-        _fmt(fmt)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (resid is not None and resid.requires_grad)):
-        return RmsNormFn.apply(x, weight, resid, eps, fmt)
-    y, h, _, _, _ = _rms_fwd(x, weight, resid, eps, 0, None, True, False, False)
-    return y if resid is None else (y, h)
+    x, resid, geom, cd = _rms_args(x, weight, resid)
+    eps = _eps(eps)
+    code, dt = (0, None) if fmt is None else _fmt(fmt)
+    if _needs_grad(x, weight, resid):
+        return RmsNormFn.apply(x, weight, resid, eps, geom, cd, code, dt)
+    y, h, _, _, _ = _rms_fwd(x, weight, resid, eps, geom, cd, 0, None, True, False)
+    return y if h is None else (y, h)
 
 
 def rms_norm8(x, weight, resid=None, eps=1e-6, fmt="e4m3"):
     """rms_norm with its output in 8 bits: Act8, or (Act8, h) with `resid`.  For inference: it carries no gradient."""
-    x, resid, eps = _rms_args(x, weight, resid, eps)
+    x, resid, geom, cd = _rms_args(x, weight, resid)
+    eps = _eps(eps)
     code, dt = _fmt(fmt)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (resid is not None and resid.requires_grad)):
+    if _needs_grad(x, weight, resid):
         raise lib.HificError("rms_norm8 carries no gradient: call it under torch.no_grad(), or rms_norm(fmt=...) in training")
-    _, h, _, q, e = _rms_fwd(x, weight, resid, eps, code, dt, False, False, True)
-    return Act8(q, e) if resid is None else (Act8(q, e), h)
+    _, h, _, q, e = _rms_fwd(x, weight, resid, eps, geom, cd, code, dt, False, False)
+    return Act8._of(q, e) if h is None else (Act8._of(q, e), h)
 
 
 # ---- channel norm with an 8-bit checkpoint ---------------------------------------------------------------------------------
-def _cn8_fwd(x, gamma, beta, resid, eps, relu, fmt):
-    code, dt = _fmt(fmt)
-    N, C, HW = _nchw(x)
+def _cn8_fwd(x, gamma, beta, resid, eps, relu, geom, cd, code, dt):
+    """-> y, rstd, q, e (normalised values), q2, e2 (y in 8 bits, with resid)."""
+    N, C, HW = geom
     y = torch.empty_like(x)
     rstd = torch.empty(_tokens(x), dtype=torch.float32, device=x.device)
     q, e = _new8(x, dt)
     q2, e2 = _new8(x, dt) if resid is not None else (None, None)
-    if x.numel():
-        call("hific_channelnorm8_fwd", ptr(x), ptr(gamma), ptr(beta), ptr(resid), ptr(y), ptr(rstd), ptr(q), ptr(e), ptr(q2),
-             ptr(e2), code, N, C, HW, eps, int(relu), lib.dtype_code(x), stream())
+    if N and HW:
+        _launch("hific_channelnorm8_fwd", x, x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), ptr(resid), y.data_ptr(), rstd.data_ptr(),
+                q.data_ptr(), e.data_ptr(), ptr(q2), ptr(e2), code, N, C, HW, eps, int(relu), cd)
     return y, rstd, q, e, q2, e2
 
 
 def _cn8_bwd(q, e, rstd, dy, gamma, beta, relu, dg, db, acc, dprev=None, acc_prev=0):
     N, C, HW = _nchw(dy)
     dx = torch.empty_like(dy)
-    if dy.numel():
+    if N and HW:
         ws, n = _bwd_ws(N, C, HW, dy.device)
-        call("hific_channelnorm8_bwd", ptr(q), ptr(e), _CODE[q.dtype], ptr(rstd), ptr(dy), ptr(gamma), ptr(beta), ptr(dx), ptr(dg),
-             ptr(db), acc, ptr(dprev), acc_prev, N, C, HW, int(relu), lib.dtype_code(dy), ptr(ws), n, stream())
+        _launch("hific_channelnorm8_bwd", dy, q.data_ptr(), e.data_ptr(), _CODE[q.dtype], rstd.data_ptr(), dy.data_ptr(), gamma.data_ptr(),
+                beta.data_ptr(), dx.data_ptr(), dg.data_ptr(), db.data_ptr(), acc, ptr(dprev), acc_prev, N, C, HW, int(relu),
+                lib.dtype_code(dy), ws.data_ptr(), n)
     else:
         for t, a in ((dg, acc), (db, acc), (dprev, acc_prev)):
             if t is not None and not a:
@@ -298,10 +318,8 @@ class ChannelNorm8Fn(Function):
     """ChannelNormFn whose backward pass reads the normalised activation in 8 bits."""
 
     @staticmethod
-    def forward(ctx, x, gamma, beta, eps, relu, resid, fmt):
-        from . import ops
-        with _on(x):
-            y, rstd, q, e, q2, e2 = _cn8_fwd(x, gamma, beta, resid, eps, relu, fmt)
+    def forward(ctx, x, gamma, beta, eps, relu, resid, geom, cd, code, dt):
+        y, rstd, q, e, q2, e2 = _cn8_fwd(x, gamma, beta, resid, eps, relu, geom, cd, code, dt)
         ctx.relu, ctx.has_resid = relu, resid is not None
         ctx.g_slot, ctx.b_slot = ops._slot(gamma), ops._slot(beta)
         ctx.save_for_backward(q, e, rstd, gamma, beta)
@@ -311,22 +329,30 @@ class ChannelNorm8Fn(Function):
         return (y,) + kept
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, _q, _e):
-        from . import ops
+        _first_order(dy)
         if dy is None:
-            return (None,) * 7
+            return (None,) * 10
         q, e, rstd, gamma, beta = ctx.saved_tensors
         dy = c16(dy)
         want = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        with _on(dy):
-            dgt, acc, dg = ops._grad_target(ctx.g_slot, gamma) if want else (torch.empty_like(gamma), 0, None)
-            dbt, acc_b, db = ops._grad_target(ctx.b_slot, beta) if want else (torch.empty_like(beta), 0, None)
-            assert acc == acc_b
-            dx = _cn8_bwd(q, e, rstd, dy, gamma, beta, ctx.relu, dgt, dbt, acc)
-            if want:
-                ops._written(ctx.g_slot, ctx.b_slot)
-        return dx, dg, db, None, None, (dy if ctx.has_resid else None), None
+        dgt, acc, dg = ops._grad_target(ctx.g_slot, gamma) if want else (torch.empty_like(gamma), 0, None)
+        dbt, acc_b, db = ops._grad_target(ctx.b_slot, beta) if want else (torch.empty_like(beta), 0, None)
+        assert acc == acc_b
+        dx = _cn8_bwd(q, e, rstd, dy, gamma, beta, ctx.relu, dgt, dbt, acc)
+        if want:
+            ops._written(ctx.g_slot, ctx.b_slot)
+        return (dx, dg, db, None, None, dy if ctx.has_resid else None) + (None,) * 4
+
+
+def _norm_args(x, gamma, beta, name):
+    geom = _nchw(x)
+    if geom[1] < 2:
+        raise lib.HificError(f"{name} needs at least two channels (unbiased variance)")
+    _one_device(x, gamma, beta)
+    _param(gamma, geom[1], "gamma")
+    _param(beta, geom[1], "beta")
+    return geom
 
 
 def channel_norm8(x, gamma, beta, eps=1e-3, relu=False, resid=None, fmt="int8"):
@@ -334,20 +360,17 @@ def channel_norm8(x, gamma, beta, eps=1e-3, relu=False, resid=None, fmt="int8"):
     gives it, and the Act8 stands for y too - what the next convolution's weight gradient reads (conv2d(x8=)).  The backward pass
     of the norm keeps its normalised input in 8 bits and nothing else of x or y.  With `relu` the kept values are on the same
     side of the ReLU as the forward values."""
-    _, C, _ = _nchw(x)
-    if C < 2:
-        raise lib.HificError("channel_norm8 needs at least two channels (unbiased variance)")
-    require_gpu_any(x, gamma, beta, resid)
-    _param(gamma, C, "gamma")
-    _param(beta, C, "beta")
-    _fmt(fmt)
+    geom = _norm_args(x, gamma, beta, "channel_norm8")
+    code, dt = _fmt(fmt)
+    cd = lib.dtype_code(x)
     if resid is not None:
+        _one_device(x, resid)
         _like(resid, x, "resid")
-        resid = _act(resid)
-    y, q, e = ChannelNorm8Fn.apply(_act(x), gamma, beta, _eps(eps), bool(relu), resid, fmt)
+        resid = c16(resid)
+    y, q, e = ChannelNorm8Fn.apply(c16(x), gamma, beta, _eps(eps), bool(relu), resid, geom, cd, code, dt)
     if resid is not None:
-        return y, Act8(q, e)
-    return y, Act8(q, e, gamma.detach(), beta.detach(), relu)
+        return y, Act8._of(q, e)
+    return y, Act8._of(q, e, gamma.detach(), beta.detach(), bool(relu))
 
 
 def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
@@ -355,20 +378,14 @@ def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
     [N, ...] the reciprocal standard deviations, dy float32 or bfloat16."""
     if not isinstance(a, Act8) or a.gamma is not None:
         raise lib.HificError("channel_norm_grad8 needs the normalised values as an Act8 without gamma / beta")
-    _, C, _ = _nchw(a.q)
-    if C < 2:
-        raise lib.HificError("channel_norm_grad8 needs at least two channels (unbiased variance)")
-    if dy.shape != a.shape:
+    _norm_args(a.q, gamma, beta, "channel_norm_grad8")
+    if dy.shape != a.q.shape:
         raise lib.HificError(f"dy must be {tuple(a.shape)}, got {tuple(dy.shape)}")
-    require_gpu_any(a.q, dy, gamma, beta, rstd)
-    _param(gamma, C, "gamma")
-    _param(beta, C, "beta")
+    _one_device(a.q, dy, rstd)
     _param(rstd, a.e.numel(), "rstd")
-    dy = _act(dy.detach())
+    lib.dtype_code(dy)
     dg, db = torch.empty_like(gamma), torch.empty_like(beta)
-    with _on(dy):
-        dx = _cn8_bwd(a.q, a.e, rstd, dy, gamma, beta, bool(relu), dg, db, 0)
-    return dx, dg, db
+    return _cn8_bwd(a.q, a.e, rstd, c16(dy.detach()), gamma, beta, bool(relu), dg, db, 0), dg, db
 
 
 # ---- weight gradients of convolutions from an 8-bit input ------------------------------------------------------------------
@@ -385,7 +402,6 @@ def _slices(N, per_sample):
 
 def _conv_wgrad8(saved, relu, dy, dw, acc, geom):
     """dw (=|+=) sum dy * pad(x), x the values of `saved` (q, e, gamma, beta) restored to dy's type."""
-    from . import ops
     q, e, gamma, beta = saved
     stride, pt, pl, pb, pr, pad_mode = geom
     N, C, H, W = q.shape
@@ -395,13 +411,12 @@ def _conv_wgrad8(saved, relu, dy, dw, acc, geom):
     for lo, hi in _slices(N, per):
         x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, dy.dtype)
         d = c16(dy[lo:hi])
-        call("hific_conv2d_bwd_weight", ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, stride, pt, pl, pb, pr, pad_mode, acc,
+        lib.call("hific_conv2d_bwd_weight", ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, stride, pt, pl, pb, pr, pad_mode, acc,
              cd, 0, *ops._ws(x), stream())
         acc = 1
 
 
 def _convt_wgrad8(saved, relu, dy, dw, acc, geom):
-    from . import ops
     q, e, gamma, beta = saved
     stride, pad, outpad = geom
     N, C, H, W = q.shape
@@ -410,7 +425,7 @@ def _convt_wgrad8(saved, relu, dy, dw, acc, geom):
     for lo, hi in _slices(N, max(C * H * W, K * dy.shape[2] * dy.shape[3])):
         x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, dy.dtype)
         d = c16(dy[lo:hi])
-        call("hific_conv_transpose2d_bwd_weight", ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, stride, pad, outpad, acc,
+        lib.call("hific_conv_transpose2d_bwd_weight", ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, stride, pad, outpad, acc,
              cd, 0, *ops._ws(x), stream())
         acc = 1
 
@@ -423,8 +438,9 @@ def _wgrad_args(a, dy, kernel, name):
     R, S = (int(k) for k in kernel)
     if R < 1 or S < 1 or R * S > 64:
         raise lib.HificError(f"{name}: kernel {(R, S)} is not supported (1 to 64 taps)")
-    require_gpu_any(a.q, dy)
-    return R, S, _act(dy.detach())
+    _one_device(a.q, dy)
+    lib.dtype_code(dy)
+    return R, S, c16(dy.detach())
 
 
 def conv2d_weight_grad8(a, dy, kernel, stride=1, pads=(0, 0, 0, 0), pad_mode=lib.PAD_ZERO):

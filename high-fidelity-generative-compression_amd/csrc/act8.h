@@ -66,6 +66,10 @@ __device__ __forceinline__ unsigned q8_next(unsigned b, bool up) {
     return FMT == HIFIC_Q_INT8 ? (unsigned)key & 0xffu : (key < 0 ? 0x80u | (unsigned)(-key) : (unsigned)key);
 }
 
+// the ReLU is open at v (at a NaN too, which then passes forward and backward)
+__device__ __forceinline__ bool relu_on(float v) { return !(v <= 0.f); }
+__device__ __forceinline__ float relu_nan(float v) { return relu_on(v) ? v : 0.f; }
+
 // xh of a norm whose ReLU follows -> 8 bits that are on the same side of the ReLU: the backward pass masks by the value that was
 // kept, and with plain rounding a fraction (step / 4) * density(0) ~ 0.3 % of int8 masks would flip - an error of 5 % (its square
 // root) in every gradient behind, ten times what the rounding itself costs.  gamma * x + beta is monotone in x, so of the two
@@ -75,10 +79,13 @@ template <int FMT>
 __device__ __forceinline__ unsigned q8_round_masked(float xh, float inv, float scale, float gamma, float beta) {
     const float t = xh * inv;
     unsigned b = q8_round<FMT>(t);
-    const float v = q8_value<FMT>(b);
-    if ((fmaf(gamma, v * scale, beta) > 0.f) != (fmaf(gamma, xh, beta) > 0.f)) b = q8_next<FMT>(b, t > v);
+    const bool on = relu_on(fmaf(gamma, xh, beta));
+    if (relu_on(fmaf(gamma, q8_value<FMT>(b) * scale, beta)) != on) b = q8_next<FMT>(b, on == (gamma > 0.f));
     return b;
 }
+
+// the compiler may not carry what it computed from r past this point
+template <typename V> __device__ __forceinline__ void forget(V& r) { asm volatile("" : "+v"(r)); }
 
 // ---- eight values at a time ------------------------------------------------------------------------------------------------
 // The wide kernels give a lane eight neighbouring values (16 bytes of bfloat16): of a plane (eight positions of a channel) or of a
@@ -87,7 +94,8 @@ __device__ __forceinline__ unsigned q8_round_masked(float xh, float inv, float s
 // end, and its first values are then computed twice, with the same result.
 typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
 typedef u32x2_t u32x2_a1 __attribute__((aligned(1)));
-typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef f32x4_t f32x4_a4 __attribute__((aligned(4)));
 
 template <typename T> struct V8;
 template <> struct V8<bf16_t> {
@@ -99,9 +107,10 @@ template <> struct V8<bf16_t> {
         for (int j = 0; j < 4; ++j) r[j] = f2bf2(v[2 * j], v[2 * j + 1]);
     }
     __device__ __forceinline__ void store(bf16_t* p) const { *(u32x4_a2*)p = r; }
+    __device__ __forceinline__ void forget() { ::forget(r); }
 };
 template <> struct V8<float> {
-    f32x4_a4 r[2];
+    f32x4_t r[2];
     __device__ __forceinline__ void load(const float* p) { r[0] = *(const f32x4_a4*)p; r[1] = *(const f32x4_a4*)(p + 4); }
     __device__ __forceinline__ float get(int j) const { return r[j >> 2][j & 3]; }
     __device__ __forceinline__ void set(const float* v) {
@@ -109,6 +118,7 @@ template <> struct V8<float> {
         for (int j = 0; j < 8; ++j) r[j >> 2][j & 3] = v[j];
     }
     __device__ __forceinline__ void store(float* p) const { *(f32x4_a4*)p = r[0]; *(f32x4_a4*)(p + 4) = r[1]; }
+    __device__ __forceinline__ void forget() { ::forget(r[0]); ::forget(r[1]); }
 };
 
 // eight values, already divided by their scales -> eight bytes.  CLAMP: only where |t| can exceed QMAX by a rounding (see q8_round).
@@ -135,74 +145,104 @@ __device__ __forceinline__ u32x2_t q8_pack8(const float* t) {
     }
     return o;
 }
-// eight bytes -> eight numbers, without the exponents
+// eight bytes -> eight values, times scale[j] (s128 = -128 * scale for int8: bytes with the sign bit flipped convert in one
+// instruction, and (u - 128) * 2^e is exact in one fused multiply-add)
 template <int FMT>
-__device__ __forceinline__ void q8_unpack8(u32x2_t q, float* v) {
+__device__ __forceinline__ void q8_unpack8(u32x2_t q, const float* scale, const float* s128, float* v) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (FMT == HIFIC_Q_INT8) {
-            const unsigned u = q[h] ^ 0x80808080u;               // unsigned bytes convert in one instruction each
+            unsigned u = q[h] ^ 0x80808080u;
+            forget(u);                                           // (or the flip is undone and redone byte by byte)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * h + j] = (float)((u >> (8 * j)) & 0xffu) - 128.f;
+            for (int j = 0; j < 4; ++j) v[4 * h + j] = fmaf((float)((u >> (8 * j)) & 0xffu), scale[4 * h + j], s128[4 * h + j]);
         } else {
             const hw_f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
-            v[4 * h] = a[0]; v[4 * h + 1] = a[1]; v[4 * h + 2] = b[0]; v[4 * h + 3] = b[1];
+            v[4 * h] = a[0] * scale[4 * h]; v[4 * h + 1] = a[1] * scale[4 * h + 1];
+            v[4 * h + 2] = b[0] * scale[4 * h + 2]; v[4 * h + 3] = b[1] * scale[4 * h + 3];
         }
     }
 }
-
-// eight normalised values whose ReLU follows (v = gamma xh + beta): q8_round_masked of each.  Without the clamp: max|xh| gave the
-// exponent, so |xh * inv| <= QMAX.
 template <int FMT>
-__device__ __forceinline__ u32x2_t q8_pack8_masked(const float* xh, const float* inv, const float* v, float gamma, float beta) {
+__device__ __forceinline__ void q8_scales(u32x2_t e, float* scale, float* s128) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const unsigned code = (e[j >> 2] >> (8 * (j & 3))) & 0xffu;
+        // (an infinite scale makes every int8 value NaN by itself: u * inf - inf)
+        scale[j] = FMT == HIFIC_Q_INT8 ? __uint_as_float(code << 23) : q8_scale(code);
+        s128[j] = FMT == HIFIC_Q_INT8 ? -128.f * scale[j] : 0.f;
+    }
+}
+
+// eight normalised values of a channel whose ReLU follows, as x = xh / scale, v = fma(gs, x, beta) with gs = gamma * scale (the
+// same product as gamma * xh): q8_round_masked of each.  No clamp: max|xh| gave the exponent, so |x| <= QMAX, and the neighbour
+// that is taken lies between x and the nearest value's other side.
+template <int FMT>
+__device__ __forceinline__ u32x2_t q8_pack8_masked(const float* x, const float* v, const float* gs, float beta, float gamma) {
+    const float up = gamma > 0.f ? 1.f : -1.f;                   // the step towards the ReLU's open side
     if (FMT == HIFIC_Q_INT8) {
         float t[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float x = xh[j] * inv[j], n = rintf(x);
-            const float scale = __uint_as_float(0x7f000000u - __float_as_uint(inv[j]));      // 1 / inv, a power of two
-            const bool wrong = (fmaf(gamma, n * scale, beta) > 0.f) != (v[j] > 0.f);
-            t[j] = wrong ? n + (x > n ? 1.f : -1.f) : n;
+            const float n = rintf(x[j]);
+            const bool on = relu_on(v[j]);
+            const float other = n + (on ? up : -up);
+            t[j] = relu_on(fmaf(gs[j], n, beta)) != on ? other : n;
         }
-        return q8_pack8<FMT, true>(t);
+        return q8_pack8<FMT, false>(t);
     }
-    float t[8];
+    u32x2_t q = q8_pack8<FMT, false>(x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = xh[j] * inv[j];
-    u32x2_t q = q8_pack8<FMT, false>(t);
-    float n[8];
-    q8_unpack8<FMT>(q, n);
+    for (int h = 0; h < 2; ++h) {
+        const hw_f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
+        const float n[4] = {a[0], a[1], b[0], b[1]};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float scale = __uint_as_float(0x7f000000u - __float_as_uint(inv[j]));
-        if ((fmaf(gamma, n[j] * scale, beta) > 0.f) != (v[j] > 0.f)) {
-            const int sh = 8 * (j & 3);
-            const unsigned b = q8_next<FMT>((q[j >> 2] >> sh) & 0xffu, t[j] > n[j]);
-            q[j >> 2] = (q[j >> 2] & ~(0xffu << sh)) | (b << sh);
+        for (int j = 0; j < 4; ++j) {
+            const bool on = relu_on(v[4 * h + j]);
+            if (relu_on(fmaf(gs[4 * h + j], n[j], beta)) != on) {
+                const unsigned c = q8_next<FMT>((q[h] >> (8 * j)) & 0xffu, (on ? up : -up) > 0.f);
+                q[h] = (q[h] & ~(0xffu << (8 * j))) | (c << (8 * j));
+            }
         }
     }
     return q;
 }
-__device__ __forceinline__ float relu_nan(float v) { return v > 0.f || v != v ? v : 0.f; }
+
+// base (the same for the whole workgroup) + a byte offset per lane: one 32-bit register addresses every tensor of a tile
+template <typename T> __device__ __forceinline__ T* at(T* base, unsigned bytes) { return (T*)((char*)base + bytes); }
+template <typename T> __device__ __forceinline__ const T* at(const T* base, unsigned bytes) { return (const T*)((const char*)base + bytes); }
 
 // Planes: lane = (group of eight positions pl = lane % LPX, channel sub-group lane / LPX).  v[j], this lane's partial of position j,
-// is combined over the 64 / LPX sub-groups of the wave: the first three steps exchange halves (4 + 2 + 1 shuffles where eight
-// separate butterflies would take 8 per step), the rest, if any, carry one value.  out[pl * 8 + j] receives the wave's result.
+// is combined over the 64 / LPX sub-groups of the wave: up to three steps exchange halves (4 + 2 + 1 shuffles where eight separate
+// butterflies would take 8 per step), further ones carry one value.  out[pl * 8 + j] receives the wave's result.
+template <int LPX, bool MAX>
+__device__ __forceinline__ unsigned tile_op(unsigned x, unsigned y) { return MAX ? umax(x, y) : x + y; }
+template <int LPX, bool MAX>
+__device__ __forceinline__ float tile_op(float x, float y) { return MAX ? fmaxf(x, y) : x + y; }
 template <int LPX, bool MAX, typename V>
 __device__ __forceinline__ void tile_reduce(const V* v, V* out) {
+    constexpr int SUBS = 64 / LPX, KEEP = SUBS >= 8 ? 1 : 8 / SUBS;      // values per lane at the end
     const int lane = threadIdx.x & 63, sub = lane / LPX;
     auto shfl = [](V x, int o) { return __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(int, x), o, 64)); };
-    auto op = [](V x, V y) { return MAX ? (x > y ? x : y) : x + y; };
-    const bool b0 = sub & 1, b1 = sub & 2, b2 = sub & 4;
-    V a[4], c[2];
+    V a[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = op(b0 ? v[4 + j] : v[j], shfl(b0 ? v[j] : v[4 + j], LPX));
+    for (int j = 0; j < 8; ++j) a[j] = v[j];
+    int first = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) c[j] = op(b1 ? a[2 + j] : a[j], shfl(b1 ? a[j] : a[2 + j], 2 * LPX));
-    V d = op(b2 ? c[1] : c[0], shfl(b2 ? c[0] : c[1], 4 * LPX));
+    for (int s = 0; s < 3; ++s) {
+        if ((1 << s) >= SUBS) break;
+        const int half = 4 >> s;
+        const bool hi = (sub >> s) & 1;
 #pragma unroll
-    for (int o = 8 * LPX; o < 64; o <<= 1) d = op(d, shfl(d, o));
-    if (sub < 8) out[(lane % LPX) * 8 + (b0 ? 4 : 0) + (b1 ? 2 : 0) + (b2 ? 1 : 0)] = d;
+        for (int j = 0; j < 4; ++j)
+            if (j < half) a[j] = tile_op<LPX, MAX>(hi ? a[half + j] : a[j], shfl(hi ? a[j] : a[half + j], LPX << s));
+        first += hi ? half : 0;
+    }
+#pragma unroll
+    for (int o = 8 * LPX; o < 64; o <<= 1) a[0] = tile_op<LPX, MAX>(a[0], shfl(a[0], o));
+    if (sub < 8)
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) out[(lane % LPX) * 8 + first + j] = a[j];
 }
 
 // Workgroups go round-robin to the 8 XCDs, each with its own L2; neighbouring tiles share 128-byte lines where a tile is narrower
@@ -212,21 +252,33 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
 }
 
 // Tile of the plane kernels: 256 threads, LPX groups of eight positions, 256 / LPX channel groups, at most `most` channels per
-// thread.  The widest LPX (8: whole 128-byte lines) that fits the channels, then narrower while the grid would not fill the
-// 256 CUs twice and a thread has more than one channel.  lpx = 0: more channels than the registers hold.
+// thread, images of less than 4 GiB.  The widest LPX that fits the channels (what a tile costs besides its values - reductions,
+// scales, barriers - is shared by most values then: norm forward 16x60x256x256 75 us, with LPX <= 8 120), then narrower while
+// there are CUs without a workgroup (16x960x16x16: 256 wide tiles 12 us, 512 narrow ones 13.4).  lpx = 0: more channels than the
+// registers hold, or images beyond 32-bit byte offsets.
 struct TileCfg { int lpx, cpt; unsigned tiles; long long blocks; };
 static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
     TileCfg t{0, 0, 0, 0};
-    for (int lpx = 8; lpx >= 1; lpx >>= 1) {
+    if ((long long)(C + 256) * HW > (1ll << 30) - 64) return t;      // (C + 256: a lane's offset is formed before it is dropped)
+    for (int lpx = 32; lpx >= 1; lpx >>= 1) {
         const int cpt = cdiv(C, 256 / lpx);
         if (cpt > most) continue;
         t.lpx = lpx; t.cpt = cpt;
         t.tiles = (unsigned)cdiv(cdiv(HW, 8), lpx);
         t.blocks = (long long)t.tiles * N;
-        if (t.blocks >= 512 || cpt <= 1) break;
+        if (t.blocks >= 256 || cpt <= 1) break;
     }
     return t;
 }
+// F(LPX, CPT) for the configuration t
+#define TILE_DISPATCH(t, MOST, F)                                                                                         \
+    do {                                                                                                                  \
+        if ((t).lpx == 32) { TILE_CPT(32, t, MOST, F); } else if ((t).lpx == 16) { TILE_CPT(16, t, MOST, F); }            \
+        else if ((t).lpx == 8) { TILE_CPT(8, t, MOST, F); } else if ((t).lpx == 4) { TILE_CPT(4, t, MOST, F); }           \
+        else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F); } else { TILE_CPT(1, t, MOST, F); }                             \
+    } while (0)
+#define TILE_CPT(LPX, t, MOST, F)                                                                                         \
+    if ((t).cpt <= 1) F(LPX, 1); else if ((t).cpt <= 2) F(LPX, 2); else if ((t).cpt <= 4) F(LPX, 4); else F(LPX, ((MOST) < 8 ? 4 : 8))
 
 // Rows: L lanes and K groups of eight channels per lane hold a row.  Sums and maxima over the row's L lanes, through LDS where a
 // row has the whole workgroup.

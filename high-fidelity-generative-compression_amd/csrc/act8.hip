@@ -35,21 +35,25 @@ __global__ __launch_bounds__(256) void act8_pack_tile_kernel(const T* __restrict
     const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / tiles, tile = bid - n * tiles;
     const unsigned oct = tile * LPX + pl, octs = ((unsigned)HW + 7) >> 3;
     const bool ok = oct < octs;
-    const unsigned hw0 = umin(ok ? oct * 8 : 0u, (unsigned)HW - 8);
-    const size_t base = (size_t)n * C * HW + hw0;
+    const unsigned hw0 = umin(ok ? oct * 8 : 0u, (unsigned)HW - 8), off = (unsigned)g * HW + hw0;
+    const unsigned kst = (unsigned)G * HW;                           // channel k of this lane: img + off + k * kst
+    const size_t img = (size_t)n * C * HW;
     V8<T> xr[CPT];
 #pragma unroll
-    for (int k = 0; k < CPT; ++k) { const int c = g + G * k; xr[k].load(x + base + (size_t)(c < C ? c : 0) * HW); }
+    for (int k = 0; k < CPT; ++k) {
+        // (channel 0 in the place of one that is not there: it counts once anyway)
+        xr[k].load(at(x + img, (g + G * k < C ? off + k * kst : hw0) * (unsigned)sizeof(T)));
+    }
     unsigned am[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) am[j] = 0;
 #pragma unroll
     for (int k = 0; k < CPT; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) am[j] = umax(am[j], g + G * k < C ? abs_bits(xr[k].get(j)) : 0u);
+        for (int j = 0; j < 8; ++j) am[j] = umax(am[j], abs_bits(xr[k].get(j)));
     tile_reduce<LPX, true>(am, red[wave]);
     __syncthreads();
-    if (tid < TP) {
+    if (tid < TP) {                      // (TP <= 256)
         const unsigned code = q8_code<FMT>(umax(umax(red[0][tid], red[1][tid]), umax(red[2][tid], red[3][tid])));
         inv_s[tid] = q8_inv_scale(code);
         const unsigned o = tile * LPX + (tid >> 3);
@@ -67,7 +71,7 @@ __global__ __launch_bounds__(256) void act8_pack_tile_kernel(const T* __restrict
             float t[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) t[j] = xr[k].get(j) * inv[j];
-            *(u32x2_a1*)(q + base + (size_t)c * HW) = q8_pack8<FMT, false>(t);
+            *(u32x2_a1*)at(q + img, off + k * kst) = q8_pack8<FMT, false>(t);
         }
     }
 }
@@ -87,26 +91,21 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const u8_t* __restric
     const int c0 = (int)(rest - img * cgs) * CH;
     const unsigned hw0 = V == 1 ? oct : umin(oct * 8, (unsigned)HW - 8);
     const size_t base = ((size_t)img * C + c0) * HW + hw0;
-    float s[V];
-    if constexpr (V == 8) {
-        const u32x2_t e = *(const u32x2_a1*)(qe + (size_t)img * HW + hw0);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = q8_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
-    } else s[0] = q8_scale(qe[(size_t)img * HW + hw0]);
+    float s[V], s128[V];
+    if constexpr (V == 8) q8_scales<FMT>(*(const u32x2_a1*)(qe + (size_t)img * HW + hw0), s, s128);
+    else s[0] = q8_scale(qe[(size_t)img * HW + hw0]);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
         if (c0 + k >= C) break;
         float v[V];
-        if constexpr (V == 8) q8_unpack8<FMT>(*(const u32x2_a1*)(q + base + (size_t)k * HW), v);
-        else v[0] = q8_value<FMT>(q[base + (size_t)k * HW]);
+        if constexpr (V == 8) q8_unpack8<FMT>(*(const u32x2_a1*)(q + base + (size_t)k * HW), s, s128, v);
+        else v[0] = q8_value<FMT>(q[base + (size_t)k * HW]) * s[0];
+        if (gamma)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            v[j] *= s[j];
-            if (gamma) {
+            for (int j = 0; j < V; ++j) {
                 v[j] = fmaf(gamma[c0 + k], v[j], beta[c0 + k]);
                 if (relu) v[j] = relu_nan(v[j]);
             }
-        }
         if constexpr (V == 8) { V8<T> o; o.set(v); o.store(out + base + (size_t)k * HW); }
         else DT<T>::st(out + base + (size_t)k * HW, v[0]);
     }
@@ -151,17 +150,16 @@ __global__ __launch_bounds__(256) void act8_restore_rows_kernel(const u8_t* __re
     if (i >= n) return;
     const long long row = i / octs;
     const unsigned c = umin((unsigned)(i - row * octs) * 8, (unsigned)C - 8);
-    const float s = q8_scale(qe[row]);
-    float v[8];
-    q8_unpack8<FMT>(*(const u32x2_a1*)(q + (size_t)row * C + c), v);
+    const unsigned e = 0x01010101u * qe[row];
+    float s[8], s128[8], v[8];
+    q8_scales<FMT>(u32x2_t{e, e}, s, s128);
+    q8_unpack8<FMT>(*(const u32x2_a1*)(q + (size_t)row * C + c), s, s128, v);
+    if (gamma)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        v[j] *= s;
-        if (gamma) {
+        for (int j = 0; j < 8; ++j) {
             v[j] = fmaf(gamma[c + j], v[j], beta[c + j]);
             if (relu) v[j] = relu_nan(v[j]);
         }
-    }
     V8<T> o; o.set(v); o.store(out + (size_t)row * C + c);
 }
 
@@ -174,9 +172,7 @@ int pack_launch(const T* x, u8_t* q, u8_t* qe, int N, int C, int HW, hipStream_t
             if (t.blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
             const dim3 grid((unsigned)t.blocks);
 #define TILE(LPX, CPT) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT>), grid, dim3(256), 0, st, x, q, qe, C, HW, t.tiles, (unsigned)t.blocks)
-#define TILE_C(LPX) do { if (t.cpt <= 1) TILE(LPX, 1); else if (t.cpt <= 2) TILE(LPX, 2); else if (t.cpt <= 4) TILE(LPX, 4); else TILE(LPX, 8); } while (0)
-            if (t.lpx == 8) TILE_C(8); else if (t.lpx == 4) TILE_C(4); else if (t.lpx == 2) TILE_C(2); else TILE_C(1);
-#undef TILE_C
+            TILE_DISPATCH(t, 8, TILE);
 #undef TILE
             return hific_launch_status();
         }

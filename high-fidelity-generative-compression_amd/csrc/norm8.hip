@@ -9,6 +9,7 @@
 // What the backward pass needs of the forward pass is xh and r: xh is kept in 8 bits (1 byte per element in the place of the 2 of
 // a bfloat16 input, or of the 4 of input and output), r in float32 per token.  Sums and statistics are float32 throughout.
 #include "act8.h"
+#include <type_traits>
 
 enum { M_RMS = 0, M_CHAN = 1 };
 enum { Q_NONE = 2 };                     // FMT of a forward kernel that writes no 8-bit tensor
@@ -42,6 +43,7 @@ struct NormFwd {
     void* y; void* h; float* rstd;
     u8_t *q, *qe, *q2, *qe2;             // xh (RMS with q_of_y: y) and, with a channel norm's resid, y
     int C, HW; unsigned tiles; float eps; int relu, q_of_y;
+    float rc, rv;                        // 1 / C, and 1 / C or 1 / (C - 1): a product in the place of a division per position
 };
 
 // Any shape: PX lanes on consecutive positions x 256 / PX channel groups, the tensor re-read by every pass (from L2).
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p) {
     if (MODE == M_CHAN) {
         float s = 0.f;
         for (int c = g; c < p.C; c += G) s += stream(c);
-        mu = tok_sum<PX>(s, red) / (float)p.C;
+        mu = tok_sum<PX>(s, red) * p.rc;
     }
     float ss = 0.f;
     for (int c = g; c < p.C; c += G) {
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p) {
         if (MODE == M_RMS && h && ok) DT<T>::st(h + c * cs, v);
     }
     ss = tok_sum<PX>(ss, red);
-    const float r = rsqrtf(ss / (float)(MODE == M_RMS ? p.C : p.C - 1) + p.eps);
+    const float r = rsqrtf(ss * p.rv + p.eps);
     if (p.rstd && ok && g == 0) p.rstd[tok] = r;
     unsigned code = 0;
     float inv = 0.f, scale = 0.f;
@@ -121,48 +123,48 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p) {
 // Planes of eight positions and more: a workgroup owns LPX * 8 positions x all channels (tile_pick), eight positions and CPT
 // channels per lane, kept as they were loaded between the passes: every tensor crosses HBM once.
 template <typename T, int MODE, int FMT, int LPX, int CPT>
-__global__ __launch_bounds__(256) void norm8_fwd_tile_kernel(const NormFwd p, unsigned blocks) {
+__global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p, unsigned blocks) {
     constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
     constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;
-    __shared__ float red[4][TP];
-    __shared__ unsigned redm[4][TP];
+    __shared__ float red[4][TP], redm[4][TP];
     __shared__ float st_r[TP], st_inv[TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
     const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / p.tiles, tile = bid - n * p.tiles;
     const unsigned oct = tile * LPX + pl, octs = ((unsigned)p.HW + 7) >> 3;
     const bool ok = oct < octs;
-    const size_t base = (size_t)n * p.C * p.HW + umin(ok ? oct * 8 : 0u, (unsigned)p.HW - 8);
+    const unsigned off0 = umin(ok ? oct * 8 : 0u, (unsigned)p.HW - 8), off = (unsigned)g * p.HW + off0;
+    const unsigned kst = (unsigned)G * p.HW;                         // channel k of this lane: img + off + k * kst
+    const size_t img = (size_t)n * p.C * p.HW;
     // position tid of the tile, for the threads that finish the statistics
     const unsigned so = tile * LPX + (tid >> 3);
     const bool sok = tid < TP && so < octs;
     const size_t stok = (size_t)n * p.HW + umin(so * 8, (unsigned)p.HW - 8) + (tid & 7);
-    const T* x = (const T*)p.x + base;
-    const T* rs = p.resid ? (const T*)p.resid + base : nullptr;
-    V8<T> xr[CPT], rr[MODE == M_CHAN ? CPT : 1];
+    const T *x = (const T*)p.x + img, *rs = (const T*)p.resid + (p.resid ? img : 0);
+    V8<T> xr[CPT], rr[CPT];
     float w[CPT], b[MODE == M_CHAN ? CPT : 1];
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
-        const int c = g + G * k, ci = c < p.C ? c : 0;
-        xr[k].load(x + (size_t)ci * p.HW);
-        w[k] = p.w[ci];
-        if constexpr (MODE == M_CHAN) { b[k] = p.b[ci]; if (rs) rr[k].load(rs + (size_t)ci * p.HW); }
+        const int c = g + G * k < p.C ? g + G * k : 0;               // (a load of channel 0 in the place of a branch around it)
+        const unsigned o = (c == 0 ? off0 : off + k * kst) * (unsigned)sizeof(T);
+        xr[k].load(at(x, o));
+        w[k] = p.w[c];
+        if constexpr (MODE == M_CHAN) b[k] = p.b[c];
+        if (p.resid) rr[k].load(at(rs, o));
     }
-    if (MODE == M_RMS && rs) {
+    if (MODE == M_RMS && p.resid) {
 #pragma unroll
         for (int k = 0; k < CPT; ++k) {
-            const int c = g + G * k, ci = c < p.C ? c : 0;
-            V8<T> a; a.load(rs + (size_t)ci * p.HW);
             float h[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = xr[k].get(j) + a.get(j);
+            for (int j = 0; j < 8; ++j) h[j] = xr[k].get(j) + rr[k].get(j);
             xr[k].set(h);
-            if (ok && c < p.C) xr[k].store((T*)p.h + base + (size_t)c * p.HW);
+            if (ok && g + G * k < p.C) xr[k].store(at((T*)p.h + img, (off + k * kst) * (unsigned)sizeof(T)));
         }
     }
-    float mu[8], acc[8];
-    unsigned am[8];
+    // maxima as floats: a NaN is lost in them, but not in the sum of squares, and r carries it into the exponent
+    float mu[8], acc[8], am[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { mu[j] = 0.f; acc[j] = 0.f; am[j] = 0; }
+    for (int j = 0; j < 8; ++j) { mu[j] = 0.f; acc[j] = 0.f; am[j] = 0.f; }
     if constexpr (MODE == M_CHAN) {
 #pragma unroll
         for (int k = 0; k < CPT; ++k)
@@ -174,11 +176,14 @@ __global__ __launch_bounds__(256) void norm8_fwd_tile_kernel(const NormFwd p, un
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = pl * 8 + j;
-            mu[j] = ((red[0][i] + red[1][i]) + (red[2][i] + red[3][i])) / (float)p.C;
+            mu[j] = ((red[0][i] + red[1][i]) + (red[2][i] + red[3][i])) * p.rc;
             acc[j] = 0.f;
         }
         __syncthreads();
     }
+    // each pass unpacks again: kept unpacked, the values would take twice the registers
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) xr[k].forget();
 #pragma unroll
     for (int k = 0; k < CPT; ++k)
         if (g + G * k < p.C)
@@ -186,86 +191,94 @@ __global__ __launch_bounds__(256) void norm8_fwd_tile_kernel(const NormFwd p, un
             for (int j = 0; j < 8; ++j) {
                 const float d = xr[k].get(j) - mu[j];
                 acc[j] += d * d;
-                if (FMT != Q_NONE) am[j] = umax(am[j], abs_bits(MODE == M_RMS && p.q_of_y ? d * w[k] : d));
+                if (FMT != Q_NONE) am[j] = fmaxf(am[j], fabsf(MODE == M_RMS && p.q_of_y ? d * w[k] : d));
             }
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) xr[k].forget();
     tile_reduce<LPX, false>(acc, red[wave]);
     if (FMT != Q_NONE) tile_reduce<LPX, true>(am, redm[wave]);
     __syncthreads();
     if (tid < TP) {
         const float ss = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
-        const float r = rsqrtf(ss / (float)(MODE == M_RMS ? p.C : p.C - 1) + p.eps);
+        const float r = rsqrtf(ss * p.rv + p.eps);
         st_r[tid] = r;
         if (p.rstd && sok) p.rstd[stok] = r;
         if (FMT != Q_NONE) {
             // max|d| r = max|d r|: a rounded product is monotone (with q_of_y the weight comes between, and q8_pack8 clamps)
-            const unsigned m = umax(umax(redm[0][tid], redm[1][tid]), umax(redm[2][tid], redm[3][tid]));
-            const unsigned code = q8_code<F>(abs_bits(__uint_as_float(m) * r));
+            const float m = fmaxf(fmaxf(redm[0][tid], redm[1][tid]), fmaxf(redm[2][tid], redm[3][tid]));
+            const unsigned code = q8_code<F>(abs_bits(m * r));
             st_inv[tid] = q8_inv_scale(code);
             if (sok) p.qe[stok] = (u8_t)code;
         }
     }
     __syncthreads();
-    float r[8], inv[8];
+    // x = d * (r / scale) is xh / scale: dividing by a power of two commutes with the rounding, and so does gs below
+    float r[8], ri[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { r[j] = st_r[pl * 8 + j]; if (FMT != Q_NONE) inv[j] = st_inv[pl * 8 + j]; am[j] = 0; }
+    for (int j = 0; j < 8; ++j) { r[j] = st_r[pl * 8 + j]; ri[j] = FMT != Q_NONE ? r[j] * st_inv[pl * 8 + j] : 0.f; am[j] = 0.f; }
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
         const int c = g + G * k;
         if (c >= p.C) continue;
-        const size_t at = base + (size_t)c * p.HW;
-        float xh[8], o[8];
+        float o[8];
+        if (MODE == M_CHAN && FMT != Q_NONE && p.relu) {
+            float x[8], gs[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            xh[j] = (xr[k].get(j) - mu[j]) * r[j];
-            o[j] = MODE == M_RMS ? xh[j] * w[k] : fmaf(w[k], xh[j], b[k]);
-        }
-        if constexpr (FMT != Q_NONE) {
-            u32x2_t q;
-            if (MODE == M_CHAN && p.relu) q = q8_pack8_masked<F>(xh, inv, o, w[k], b[k]);
-            else {
+            for (int j = 0; j < 8; ++j) {
+                // 1 / inv, a power of two (2^127 for a token that is not finite: its values are NaN)
+                gs[j] = w[k] * __uint_as_float(0x7f000000u - __float_as_uint(st_inv[pl * 8 + j]));
+                x[j] = (xr[k].get(j) - mu[j]) * ri[j];
+                o[j] = fmaf(gs[j], x[j], b[MODE == M_CHAN ? k : 0]);
+            }
+            const u32x2_t q = q8_pack8_masked<F>(x, o, gs, b[MODE == M_CHAN ? k : 0], w[k]);
+            if (ok) *(u32x2_a1*)at(p.q + img, off + k * kst) = q;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float xh = (xr[k].get(j) - mu[j]) * r[j];
+                o[j] = MODE == M_RMS ? xh * w[k] : fmaf(w[k], xh, b[MODE == M_CHAN ? k : 0]);
+            }
+            if constexpr (FMT != Q_NONE) {
                 float t[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) t[j] = (MODE == M_RMS && p.q_of_y ? o[j] : xh[j]) * inv[j];
-                q = q8_pack8<F, MODE == M_RMS>(t);
+                for (int j = 0; j < 8; ++j)
+                    t[j] = MODE == M_RMS && p.q_of_y ? o[j] * st_inv[pl * 8 + j] : (xr[k].get(j) - mu[j]) * ri[j];
+                const u32x2_t q = q8_pack8<F, MODE == M_RMS>(t);
+                if (ok) *(u32x2_a1*)at(p.q + img, off + k * kst) = q;
             }
-            if (ok) *(u32x2_a1*)(p.q + at) = q;
         }
         if constexpr (MODE == M_CHAN) {
             if (p.relu)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = relu_nan(o[j]);
-            if (rs) {                    // both terms rounded to the storage type first, as norm and add one after the other
+            if (p.resid) {               // both terms rounded to the storage type first, as norm and add one after the other
                 V8<T> t; t.set(o);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { o[j] = t.get(j) + rr[k].get(j); if (FMT != Q_NONE) am[j] = umax(am[j], abs_bits(o[j])); }
-                if (p.q2) {              // the sum replaces x: kept in float32 precision by its two terms until the exponent is known
-                    xr[k] = t;
-                }
+                for (int j = 0; j < 8; ++j) { o[j] = t.get(j) + rr[k].get(j); if (FMT != Q_NONE) am[j] = fmaxf(am[j], fabsf(o[j])); if (o[j] != o[j]) am[j] = INFINITY; }
+                xr[k] = t;               // q2 below: the sum again from its two terms, in float32
             }
         }
-        if (p.y && ok) { V8<T> t; t.set(o); t.store((T*)p.y + at); }
+        if (p.y && ok) { V8<T> t; t.set(o); t.store(at((T*)p.y + img, (off + k * kst) * (unsigned)sizeof(T))); }
     }
     if constexpr (MODE == M_CHAN && FMT != Q_NONE) {
         if (!p.q2) return;
-        tile_reduce<LPX, true>(am, redm[wave]);          // (its readers of the first maximum are behind two barriers)
+        tile_reduce<LPX, true>(am, redm[wave]);          // (a NaN as an infinity; redm's readers are behind a barrier)
         __syncthreads();
         if (tid < TP) {
-            const unsigned code = q8_code<F>(umax(umax(redm[0][tid], redm[1][tid]), umax(redm[2][tid], redm[3][tid])));
+            const unsigned code = q8_code<F>(abs_bits(fmaxf(fmaxf(redm[0][tid], redm[1][tid]), fmaxf(redm[2][tid], redm[3][tid]))));
             st_inv[tid] = q8_inv_scale(code);
             if (sok) p.qe2[stok] = (u8_t)code;
         }
         __syncthreads();
         if (!ok) return;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) inv[j] = st_inv[pl * 8 + j];
-#pragma unroll
         for (int k = 0; k < CPT; ++k) {
             const int c = g + G * k;
             if (c >= p.C) continue;
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (xr[k].get(j) + rr[k].get(j)) * inv[j];
-            *(u32x2_a1*)(p.q2 + base + (size_t)c * p.HW) = q8_pack8<F, false>(t);
+            for (int j = 0; j < 8; ++j) t[j] = (xr[k].get(j) + rr[k].get(j)) * st_inv[pl * 8 + j];
+            *(u32x2_a1*)at(p.q2 + img, off + k * kst) = q8_pack8<F, false>(t);
         }
     }
 }
@@ -288,8 +301,7 @@ __global__ __launch_bounds__(256) void rms_fwd_rows_kernel(const NormFwd p, int 
         if (p.resid) rr[k].load((const T*)p.resid + base + c);
         w[k].load(p.w + c);
     }
-    float ss = 0.f;
-    unsigned am = 0;
+    float ss = 0.f, am = 0.f;            // (a NaN is lost in am, not in ss, and r carries it into the exponent)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const unsigned cn = (unsigned)(l + L * k) * 8, c = umin(cn, C - 8);
@@ -305,14 +317,14 @@ __global__ __launch_bounds__(256) void rms_fwd_rows_kernel(const NormFwd p, int 
             // a group past the end was moved back: its first values belong to the group before it
             const float v = c + j >= cn ? xr[k].get(j) : 0.f;
             ss += v * v;
-            if (FMT != Q_NONE) am = umax(am, abs_bits(p.q_of_y ? v * w[k].get(j) : v));
+            if (FMT != Q_NONE) am = fmaxf(am, fabsf(p.q_of_y ? v * w[k].get(j) : v));
         }
     }
     ss = row_sum<L>(ss);
-    const float r = rsqrtf(ss / (float)C + p.eps);
+    const float r = rsqrtf(ss * p.rv + p.eps);
     float inv = 0.f;
     if constexpr (FMT != Q_NONE) {
-        const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(am)) * r));
+        const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(__float_as_uint(am))) * r));
         inv = q8_inv_scale(code);
         if (ok && l == 0) p.qe[row0] = (u8_t)code;
     }
@@ -342,6 +354,7 @@ struct NormBwd {
     void* dx; float* part;
     int C, HW; unsigned tiles; int relu, db;
     long long tokens; int nsplit;
+    float rc, rv;                        // as in NormFwd
 };
 
 template <typename T, int SRC>
@@ -365,17 +378,17 @@ __global__ __launch_bounds__(256) void norm8_bwd_kernel(const NormBwd p) {
     for (int c = g; c < p.C; c += G) {
         const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
         float d = DT<T>::ld(dy + c * cs);
-        if (MODE == M_CHAN && p.relu && !(fmaf(p.w[c], xh, p.b[c]) > 0.f)) d = 0.f;
+        if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
         d *= p.w[c];
         s1 += d; s2 += d * xh;
     }
-    if (MODE == M_CHAN) s1 = tok_sum<PX>(s1, red) / (float)p.C;
-    s2 = tok_sum<PX>(s2, red) / (float)(MODE == M_RMS ? p.C : p.C - 1);
+    if (MODE == M_CHAN) s1 = tok_sum<PX>(s1, red) * p.rc;
+    s2 = tok_sum<PX>(s2, red) * p.rv;
     if (!ok) return;
     for (int c = g; c < p.C; c += G) {
         const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
         float d = DT<T>::ld(dy + c * cs);
-        if (MODE == M_CHAN && p.relu && !(fmaf(p.w[c], xh, p.b[c]) > 0.f)) d = 0.f;
+        if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
         d = d * p.w[c] - xh * s2;
         if (MODE == M_CHAN) d -= s1;
         d *= r;
@@ -397,7 +410,7 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
             const size_t i = ((size_t)n * p.C + c) * p.HW + (t - n * p.HW);
             const float xh = norm8_xh<T, SRC>(p, i, p.rstd[t], SRC == SRC_T ? 0.f : q8_scale(p.qe[t]));
             float d = DT<T>::ld((const T*)p.dy + i);
-            if (MODE == M_CHAN && p.relu && !(fmaf(p.w[c], xh, p.b[c]) > 0.f)) d = 0.f;
+            if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
             sg += d * xh; sb += d;
             if (MODE == M_CHAN && p.db) sd += DT<T>::ld((const T*)p.dx + i);
         }
@@ -416,13 +429,15 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
 // Planes: as norm8_fwd_tile_kernel.  A workgroup takes `pit` tiles of one image in turn and keeps the sums of its channels in
 // registers: part[workgroup][0..2][c] as norm8_param_kernel.
 template <typename T, int MODE, int SRC, int LPX, int CPT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
+__global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
     constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
     __shared__ float red[2][4][TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
     const unsigned per = (p.tiles + pit - 1) / pit;                  // workgroups per image
     const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / per, t0 = (bid - n * per) * pit;
     const unsigned octs = ((unsigned)p.HW + 7) >> 3;
+    const unsigned kst = (unsigned)G * p.HW;                         // channel k of this lane: img + off + k * kst
+    const size_t img = (size_t)n * p.C * p.HW;
     float w[CPT], b[MODE == M_CHAN ? CPT : 1], pg[CPT], pb[MODE == M_CHAN ? CPT : 1], pd[MODE == M_CHAN ? CPT : 1];
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
@@ -435,57 +450,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
         const bool ok = oct < octs;
         const unsigned hw0 = umin(ok ? oct * 8 : 0u, (unsigned)p.HW - 8);
         const int dup = ok ? (int)(oct * 8 - hw0) : 8;               // values that another lane adds to the channels' sums
-        const size_t base = (size_t)n * p.C * p.HW + hw0, tok = (size_t)n * p.HW + hw0;
+        const unsigned off = (unsigned)g * p.HW + hw0;
+        const size_t tok = (size_t)n * p.HW + hw0;
         V8<T> dy[CPT], hr[SRC == SRC_T ? CPT : 1], ds[MODE == M_RMS ? CPT : 1];
         u32x2_t q[SRC == SRC_T ? 1 : CPT];
 #pragma unroll
         for (int k = 0; k < CPT; ++k) {
-            const int c = g + G * k;
-            const size_t at = base + (size_t)(c < p.C ? c : 0) * p.HW;
-            if constexpr (SRC == SRC_T) hr[k].load((const T*)p.h + at); else q[k] = *(const u32x2_a1*)(p.q + at);
-            dy[k].load((const T*)p.dy + at);
-            if constexpr (MODE == M_RMS) if (p.dstream) ds[k].load((const T*)p.dstream + at);
+            const unsigned o = g + G * k < p.C ? off + k * kst : hw0, oT = o * (unsigned)sizeof(T);
+            if constexpr (SRC == SRC_T) hr[k].load(at((const T*)p.h + img, oT));
+            else q[k] = *(const u32x2_a1*)at(p.q + img, o);
+            dy[k].load(at((const T*)p.dy + img, oT));
+            if constexpr (MODE == M_RMS) if (p.dstream) ds[k].load(at((const T*)p.dstream + img, oT));
         }
         V8<float> r; r.load(p.rstd + tok);
-        float sc[8];
-        if constexpr (SRC == SRC_T) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[j] = r.get(j);
-        } else {
-            const u32x2_t e = *(const u32x2_a1*)(p.qe + tok);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sc[j] = q8_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
-        }
+        float sc[8], s128[8];
+        if constexpr (SRC != SRC_T) q8_scales<SRC>(*(const u32x2_a1*)(p.qe + tok), sc, s128);
         auto values = [&](int k, float* xh) {
             if constexpr (SRC == SRC_T) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * sc[j];
-            } else {
-                q8_unpack8<SRC>(q[k], xh);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) xh[j] *= sc[j];
-            }
+                for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * r.get(j);
+            } else q8_unpack8<SRC>(q[k], sc, s128, xh);
         };
         float s1[8], s2[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) { s1[j] = 0.f; s2[j] = 0.f; }
+        auto sums = [&](auto moved) {    // moved: this lane's group was moved back at the plane's end, or is not there
 #pragma unroll
-        for (int k = 0; k < CPT; ++k) {
-            if (g + G * k >= p.C) continue;
-            float xh[8];
-            values(k, xh);
+            for (int k = 0; k < CPT; ++k) {
+                if (g + G * k >= p.C) continue;
+                float xh[8];
+                values(k, xh);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float d = dy[k].get(j);
-                if (MODE == M_CHAN && p.relu && !(fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]) > 0.f)) d = 0.f;
-                const float dk = j >= dup ? d : 0.f;
-                pg[k] += dk * xh[j];
-                if constexpr (MODE == M_CHAN) pb[k] += dk;
-                d *= w[k];
-                if (MODE == M_CHAN) s1[j] += d;
-                s2[j] += d * xh[j];
+                for (int j = 0; j < 8; ++j) {
+                    float d = dy[k].get(j);
+                    if (MODE == M_CHAN && p.relu && !relu_on(fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]))) d = 0.f;
+                    const float dk = decltype(moved)::value && j < dup ? 0.f : d;
+                    pg[k] += dk * xh[j];
+                    if constexpr (MODE == M_CHAN) pb[k] += dk;
+                    d *= w[k];
+                    if (MODE == M_CHAN) s1[j] += d;
+                    s2[j] += d * xh[j];
+                }
             }
-        }
+        };
+        if (__any(dup != 0)) sums(std::true_type{}); else sums(std::false_type{});
+        // the second pass unpacks again: kept unpacked, the values of more than two channels would cost waves
+        if constexpr (CPT > 2)
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) { dy[k].forget(); if constexpr (SRC == SRC_T) hr[k].forget(); else forget(q[k]); }
         if (it > 0) __syncthreads();                                 // the readers of the previous tile's sums are done
         tile_reduce<LPX, false>(s2, red[1][wave]);
         if (MODE == M_CHAN) tile_reduce<LPX, false>(s1, red[0][wave]);
@@ -493,8 +505,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int i = pl * 8 + j;
-            s2[j] = ((red[1][0][i] + red[1][1][i]) + (red[1][2][i] + red[1][3][i])) / (float)(MODE == M_RMS ? p.C : p.C - 1);
-            if (MODE == M_CHAN) s1[j] = ((red[0][0][i] + red[0][1][i]) + (red[0][2][i] + red[0][3][i])) / (float)p.C;
+            s2[j] = ((red[1][0][i] + red[1][1][i]) + (red[1][2][i] + red[1][3][i])) * p.rv;
+            if (MODE == M_CHAN) s1[j] = ((red[0][0][i] + red[0][1][i]) + (red[0][2][i] + red[0][3][i])) * p.rc;
         }
 #pragma unroll
         for (int k = 0; k < CPT; ++k) {
@@ -505,14 +517,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void n
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float d = dy[k].get(j);
-                if (MODE == M_CHAN && p.relu && !(fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]) > 0.f)) d = 0.f;
+                if (MODE == M_CHAN && p.relu && !relu_on(fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]))) d = 0.f;
                 d = d * w[k] - xh[j] * s2[j];
                 if (MODE == M_CHAN) d -= s1[j];
                 o[j] = d * r.get(j);
                 if constexpr (MODE == M_RMS) if (p.dstream) o[j] += ds[k].get(j);
             }
             V8<T> t; t.set(o);
-            if (ok) t.store((T*)p.dx + base + (size_t)c * p.HW);
+            if (ok) t.store(at((T*)p.dx + img, (off + k * kst) * (unsigned)sizeof(T)));
             if constexpr (MODE == M_CHAN)
                 if (p.db)
 #pragma unroll
@@ -564,17 +576,13 @@ __global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int 
             if (p.dstream) ds[k].load((const T*)p.dstream + at);
         }
         const float r = p.rstd[row];
-        float sc = r;
-        if constexpr (SRC != SRC_T) sc = q8_scale(p.qe[row]);
+        float sc[8], s128[8];
+        if constexpr (SRC != SRC_T) { const unsigned e = 0x01010101u * p.qe[row]; q8_scales<SRC>(u32x2_t{e, e}, sc, s128); }
         auto values = [&](int k, float* xh) {
             if constexpr (SRC == SRC_T) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * sc;
-            } else {
-                q8_unpack8<SRC>(q[k], xh);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) xh[j] *= sc;
-            }
+                for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * r;
+            } else q8_unpack8<SRC>(q[k], sc, s128, xh);
         };
         float s2 = 0.f;
 #pragma unroll
@@ -589,7 +597,7 @@ __global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int 
                 s2 += d * w[k].get(j);
             }
         }
-        s2 = row_sum<L>(s2) / (float)C;
+        s2 = row_sum<L>(s2) * p.rv;
         if (!ok) continue;               // (only the last round has rows that are not there, and none of its lanes waits again)
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -630,30 +638,36 @@ __global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int 
     }
 }
 
-// column sums of part[rows][nr * C] into up to three vectors, each written or added to: 64 columns x 16 row lanes, fixed order
+// column sums of part[rows][nr * C] into up to three vectors, each written or added to, in a fixed order: 16 columns x 64 row
+// lanes per workgroup (a few hundred columns of ~1000 rows: more row lanes, so that no thread adds more than a few dozen)
 __global__ __launch_bounds__(1024) void norm8_colsum_kernel(const float* __restrict__ part, float* __restrict__ d0, float* __restrict__ d1,
                                                             float* __restrict__ d2, int C, int rows, int nr, int acc, int acc2) {
-    __shared__ float red[16][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6, W = nr * C;
+    __shared__ float red[64][17];
+    const int cl = threadIdx.x & 15, col = blockIdx.x * 16 + cl, rl = threadIdx.x >> 4, W = nr * C;
     float s = 0.f;
     if (col < W) {
         int r = rl;
-        for (; r + 112 < rows; r += 128) {
+        for (; r + 448 < rows; r += 512) {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = part[(size_t)(r + 16 * j) * W + col];
+            for (int j = 0; j < 8; ++j) v[j] = part[(size_t)(r + 64 * j) * W + col];
             s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
-        for (; r < rows; r += 16) s += part[(size_t)r * W + col];
+        for (; r < rows; r += 64) s += part[(size_t)r * W + col];
     }
-    red[rl][threadIdx.x & 63] = s;
+    red[rl][cl] = s;
     __syncthreads();
-    if (rl == 0 && col < W) {
+    if (threadIdx.x < 64) {
+        const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
         float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x & 63];
-        float* d = col < C ? d0 + col : (col < 2 * C ? d1 + (col - C) : d2 + (col - 2 * C));
-        if (col < 2 * C ? acc : acc2) *d += t; else *d = t;
+        for (int i = 0; i < 16; ++i) t += red[q * 16 + i][c];
+        t += __shfl_xor(t, 16, 64);
+        t += __shfl_xor(t, 32, 64);
+        if (q == 0 && col < W) {
+            float* d = col < C ? d0 + col : (col < 2 * C ? d1 + (col - C) : d2 + (col - 2 * C));
+            if (col < 2 * C ? acc : acc2) *d += t; else *d = t;
+        }
     }
 }
 
@@ -666,18 +680,19 @@ int norm8_nsplit(int N, int C, int HW) {                             // ~1024 wo
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s);
 }
-// tiles per workgroup of the backward plane kernel: ~2048 workgroups, so that few rows of channel sums are written
+// tiles per workgroup of the backward plane kernel: 512 workgroups, two per CU (what its registers allow), each with its share of
+// the tiles - one round, few rows of channel sums (16x120x128x128: 43 us, with 1024 workgroups 47.5, with 2048 53)
 unsigned norm8_pit(const TileCfg& t, long long N) {
-    unsigned pit = (unsigned)(t.blocks / 2048);
+    unsigned pit = (unsigned)(t.blocks / 512);
     return pit < 1 ? 1 : (pit > t.tiles ? t.tiles : pit);
 }
-// channels per thread that the forward / backward plane kernels keep in registers
-template <typename T> constexpr int tile_most(bool bwd) { return sizeof(T) == 2 ? 8 : (bwd ? 4 : 8); }
+// channels per thread that the plane kernels keep in registers
+template <typename T> constexpr int tile_most() { return sizeof(T) == 2 ? 8 : 4; }
 // rows of channel sums that the backward pass writes
 template <typename T>
 size_t norm8_rows(int mode, int N, int C, int HW) {
     if (HW >= 8) {
-        const TileCfg t = tile_pick(N, C, HW, tile_most<T>(true));
+        const TileCfg t = tile_pick(N, C, HW, tile_most<T>());
         if (t.lpx) return (size_t)cdiv((int)t.tiles, (int)norm8_pit(t, N)) * N;
     }
     if (mode == M_RMS && HW == 1 && C >= 8) {
@@ -687,23 +702,17 @@ size_t norm8_rows(int mode, int N, int C, int HW) {
     return (size_t)norm8_nsplit(N, C, HW);
 }
 
-#define NORM8_TILE(T, t, F)                                                                                               \
-    do {                                                                                                                  \
-        if ((t).lpx == 8) { NORM8_CPT(T, 8, t, F); } else if ((t).lpx == 4) { NORM8_CPT(T, 4, t, F); }                    \
-        else if ((t).lpx == 2) { NORM8_CPT(T, 2, t, F); } else { NORM8_CPT(T, 1, t, F); }                                 \
-    } while (0)
-#define NORM8_CPT(T, LPX, t, F)                                                                                           \
-    if ((t).cpt <= 1) F(LPX, 1); else if ((t).cpt <= 2) F(LPX, 2); else if ((t).cpt <= 4) F(LPX, 4); else F(LPX, 8)
-
 template <typename T, int MODE, int FMT>
 int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
+    p.rc = 1.f / (float)p.C;
+    p.rv = 1.f / (float)(MODE == M_RMS ? p.C : p.C - 1);
     if (p.HW >= 8) {
-        const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>(false));
+        const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>());
         if (t.lpx) {
             if (t.blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
             p.tiles = t.tiles;
 #define FWD(LPX, CPT) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, LPX, CPT>), dim3((unsigned)t.blocks), dim3(256), 0, st, p, (unsigned)t.blocks)
-            NORM8_TILE(T, t, FWD);
+            TILE_DISPATCH(t, tile_most<T>(), FWD);
 #undef FWD
             return hific_launch_status();
         }
@@ -730,24 +739,21 @@ int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
 
 template <typename T, int MODE, int SRC>
 int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc, int acc2, size_t ws_bytes, hipStream_t st) {
+    p.rc = 1.f / (float)p.C;
+    p.rv = 1.f / (float)(MODE == M_RMS ? p.C : p.C - 1);
     const int nr = MODE == M_RMS ? 1 : 2 + p.db;
     const size_t rows = norm8_rows<T>(MODE, N, p.C, p.HW);
     if (rows * nr * p.C * sizeof(float) > ws_bytes) return HIFIC_ERR_WS;
     TileCfg t{0, 0, 0, 0};
     RowCfg r{0, 0};
-    if (p.HW >= 8) t = tile_pick(N, p.C, p.HW, tile_most<T>(true));
+    if (p.HW >= 8) t = tile_pick(N, p.C, p.HW, tile_most<T>());
     else if (MODE == M_RMS && p.HW == 1 && p.C >= 8) r = row_pick(N, p.C);
     if (rows > 0x7fffffffull) return HIFIC_ERR_UNSUPPORTED;
     if (t.lpx) {
         p.tiles = t.tiles;
         const unsigned pit = norm8_pit(t, N);
 #define BWD(LPX, CPT) hipLaunchKernelGGL((norm8_bwd_tile_kernel<T, MODE, SRC, LPX, CPT>), dim3((unsigned)rows), dim3(256), 0, st, p, (unsigned)rows, pit)
-        if constexpr (tile_most<T>(true) == 8) NORM8_TILE(T, t, BWD);
-        else {
-#undef NORM8_CPT
-#define NORM8_CPT(T, LPX, t, F) if ((t).cpt <= 1) F(LPX, 1); else if ((t).cpt <= 2) F(LPX, 2); else F(LPX, 4)
-            NORM8_TILE(T, t, BWD);
-        }
+        TILE_DISPATCH(t, tile_most<T>(), BWD);
 #undef BWD
     } else if (r.l) {
         if constexpr (MODE == M_RMS) {
@@ -771,7 +777,7 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
         if (px == 1) BWD(1); else if (px == 16) BWD(16); else BWD(64);
 #undef BWD
     }
-    hipLaunchKernelGGL(norm8_colsum_kernel, dim3(cdiv(nr * p.C, 64)), dim3(1024), 0, st, p.part, d0, d1, d2, p.C, (int)rows, nr, acc, acc2);
+    hipLaunchKernelGGL(norm8_colsum_kernel, dim3(cdiv(nr * p.C, 16)), dim3(1024), 0, st, p.part, d0, d1, d2, p.C, (int)rows, nr, acc, acc2);
     return hific_launch_status();
 }
 }  // namespace
@@ -783,7 +789,7 @@ int hific_rms_norm_fwd(const void* x, const void* resid, const float* w, void* y
     if (!x || !w || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype) || !(eps > 0.f)) return HIFIC_ERR_ARG;
     if ((resid != nullptr) != (h != nullptr) || (q != nullptr) != (qe != nullptr) || (!y && !q)) return HIFIC_ERR_ARG;
     if (q && !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
-    NormFwd p{x, resid, w, nullptr, y, h, rstd, (u8_t*)q, (u8_t*)qe, nullptr, nullptr, C, HW, 0, eps, 0, q_of_y};
+    NormFwd p{x, resid, w, nullptr, y, h, rstd, (u8_t*)q, (u8_t*)qe, nullptr, nullptr, C, HW, 0, eps, 0, q_of_y, 0.f, 0.f};
 #define RMS(T) (!q ? norm8_fwd_launch<T, M_RMS, Q_NONE>(p, N, st) : fmt == HIFIC_Q_INT8                                     \
                    ? norm8_fwd_launch<T, M_RMS, HIFIC_Q_INT8>(p, N, st) : norm8_fwd_launch<T, M_RMS, HIFIC_Q_E4M3>(p, N, st))
     return dtype == HIFIC_F32 ? RMS(float) : RMS(bf16_t);
@@ -806,7 +812,7 @@ int hific_rms_norm_bwd(const void* h, const void* q, const void* qe, int fmt, co
                        hipStream_t st) {
     if (!rstd || !dy || !w || !dx || !dw || !ws || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype)) return HIFIC_ERR_ARG;
     if ((h != nullptr) == (q != nullptr) || (q != nullptr) != (qe != nullptr) || (q && !act8_fmt_ok(fmt))) return HIFIC_ERR_ARG;
-    NormBwd p{h, (const u8_t*)q, (const u8_t*)qe, rstd, dy, dstream, w, nullptr, dx, (float*)ws, C, HW, 0, 0, 0, 0, 0};
+    NormBwd p{h, (const u8_t*)q, (const u8_t*)qe, rstd, dy, dstream, w, nullptr, dx, (float*)ws, C, HW, 0, 0, 0, 0, 0, 0.f, 0.f};
 #define RMS(T) (h ? norm8_bwd_launch<T, M_RMS, SRC_T>(p, N, dw, nullptr, nullptr, accumulate, 0, ws_bytes, st)              \
                   : fmt == HIFIC_Q_INT8                                                                                     \
                   ? norm8_bwd_launch<T, M_RMS, HIFIC_Q_INT8>(p, N, dw, nullptr, nullptr, accumulate, 0, ws_bytes, st)       \
@@ -820,7 +826,7 @@ int hific_channelnorm8_fwd(const void* x, const float* gamma, const float* beta,
     if (!x || !gamma || !beta || !y || !rstd || !q || !qe || N <= 0 || C < 2 || HW <= 0 || !(eps > 0.f)) return HIFIC_ERR_ARG;
     if (!act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
     if ((q2 != nullptr) != (qe2 != nullptr) || (q2 && !resid)) return HIFIC_ERR_ARG;
-    NormFwd p{x, resid, gamma, beta, y, nullptr, rstd, (u8_t*)q, (u8_t*)qe, (u8_t*)q2, (u8_t*)qe2, C, HW, 0, eps, relu, 0};
+    NormFwd p{x, resid, gamma, beta, y, nullptr, rstd, (u8_t*)q, (u8_t*)qe, (u8_t*)q2, (u8_t*)qe2, C, HW, 0, eps, relu, 0, 0.f, 0.f};
 #define CN(T) (fmt == HIFIC_Q_INT8 ? norm8_fwd_launch<T, M_CHAN, HIFIC_Q_INT8>(p, N, st) : norm8_fwd_launch<T, M_CHAN, HIFIC_Q_E4M3>(p, N, st))
     return dtype == HIFIC_F32 ? CN(float) : CN(bf16_t);
 #undef CN
@@ -832,7 +838,7 @@ int hific_channelnorm8_bwd(const void* q, const void* qe, int fmt, const float* 
     if (!q || !qe || !rstd || !dy || !gamma || !beta || !dx || !dgamma || !dbeta || !ws || N <= 0 || C < 2 || HW <= 0) return HIFIC_ERR_ARG;
     if (!act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
     NormBwd p{nullptr, (const u8_t*)q, (const u8_t*)qe, rstd, dy, nullptr, gamma, beta, dx, (float*)ws, C, HW, 0, relu,
-              dprev_bias ? 1 : 0, 0, 0};
+              dprev_bias ? 1 : 0, 0, 0, 0.f, 0.f};
 #define CN(T) (fmt == HIFIC_Q_INT8                                                                                                       \
                    ? norm8_bwd_launch<T, M_CHAN, HIFIC_Q_INT8>(p, N, dgamma, dbeta, dprev_bias, accumulate, accumulate_prev, ws_bytes, st) \
                    : norm8_bwd_launch<T, M_CHAN, HIFIC_Q_E4M3>(p, N, dgamma, dbeta, dprev_bias, accumulate, accumulate_prev, ws_bytes, st))

@@ -430,10 +430,37 @@ def test_refusals_on_the_device(hific, dev):
         with pytest.raises(lib.HificError):
             f()
             pytest.fail(f"refusal {i} was accepted")
-    y = ops.rms_norm(x.clone().requires_grad_(), w)
-    g, = torch.autograd.grad(y, y.grad_fn.next_functions[0][0].variable, torch.ones_like(y), create_graph=True)
+    xd = x.clone().requires_grad_()
+    g, = torch.autograd.grad(ops.rms_norm(xd, w), xd, torch.ones_like(x), create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()                               # no second derivative, and it says so
+    for f in (lambda: ops.rms_norm(xd, w), lambda: ops.channel_norm8(xd, w, w)[0]):
+        with pytest.raises(lib.HificError):
+            torch.autograd.grad(f().square().sum(), xd, create_graph=True)
+
+
+@pytest.mark.parametrize("shape", [(5, 24), (5, 21), (2, 24, 3, 8), (2, 20, 3, 5), (2, 20, 1, 3)])
+def test_tokens_that_are_not_finite_stay_so_and_alone(hific, dev, shape):
+    """An infinity or NaN in a token: its 8-bit form restores to NaN, its gradient is NaN; the other tokens are as without it."""
+    from hific_amd import ops
+    x, w, b, dy = _rand(shape, 181), _chan(shape, 182), _chan(shape, 183, 0.0), _rand(shape, 184)
+    flat = x.movedim(1, -1).reshape(-1, shape[1]).clone()
+    flat[0, 3], flat[1, 7] = float("inf"), float("nan")
+    bad = flat.reshape(shape[:1] + shape[2:] + shape[1:2]).movedim(-1, 1).contiguous()
+    hit = ~torch.isfinite(bad).all(1, keepdim=True).expand(shape)
+    for fmt in ("int8", "e4m3"):
+        outs = []
+        for v in (x, bad):
+            xd = v.to(dev).requires_grad_()
+            y, a = ops.channel_norm8(xd, w.to(dev), b.to(dev), relu=True, fmt=fmt)
+            dx, = torch.autograd.grad(y, xd, dy.to(dev))
+            z, c = ops.channel_norm8(v.to(dev), w.to(dev), b.to(dev), resid=v.to(dev), fmt=fmt)
+            xr = v.to(dev).requires_grad_()
+            dr, = torch.autograd.grad(ops.rms_norm(xr, w.to(dev), fmt=fmt), xr, dy.to(dev))
+            outs.append([t.detach().cpu() for t in (y, ops.restore8(a), dx, z, ops.restore8(c), dr, ops.restore8(ops.rms_norm8(v.to(dev), w.to(dev), fmt=fmt)))])
+        for i, (good, got) in enumerate(zip(*outs)):
+            assert torch.isnan(got[hit]).all(), (fmt, i)
+            assert torch.equal(got[~hit], good[~hit]), (fmt, i)
 
 
 def test_kept_tensors_are_guarded_against_changes_in_place(hific, dev):
