@@ -8,6 +8,7 @@ and `conv2d_weight_grad8` / `conv_transpose2d_weight_grad8` contract one.  The f
 """
 import contextlib
 import functools
+import os
 
 import torch
 from torch.autograd import Function
@@ -388,6 +389,232 @@ def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
     return _cn8_bwd(a.q, a.e, rstd, c16(dy.detach()), gamma, beta, bool(relu), dg, db, 0), dg, db
 
 
+# ---- training with 8-bit checkpoints ---------------------------------------------------------------------------------------------
+# Every conv -> ChannelNorm block of the Generator (and of the Encoder where it runs the plain chain) keeps, for its backward pass,
+# the normalised values in 8 bits and nothing else: they serve the norm's own backward pass and, with gamma / beta, stand for the
+# block's output in the next convolution's weight gradient - 1 byte per element in the place of two bfloat16 tensors (4).
+# HIFIC_CHECKPOINT8=int8|e4m3 / hific_amd.set_checkpoint8(...); off by default.
+_CHECKPOINT8 = os.environ.get("HIFIC_CHECKPOINT8", "") or None
+if _CHECKPOINT8 is not None:
+    _fmt(_CHECKPOINT8)
+
+
+def set_checkpoint8(fmt):
+    """"int8" | "e4m3": training forwards keep 8-bit activations (see above); None: bfloat16 / float32 ones."""
+    global _CHECKPOINT8
+    if fmt is not None:
+        _fmt(fmt)
+    _CHECKPOINT8 = fmt
+
+
+def checkpoint8_fmt():
+    return _CHECKPOINT8
+
+
+def _conv_geom(x, weight, geom):
+    """(N, C, H, W, K, R, S, OH, OW); geom of 3 entries: nn.ConvTranspose2d, of 6: nn.Conv2d."""
+    N, C, H, W = x.shape
+    if len(geom) == 3:
+        stride, pad, outpad = geom
+        Cw, K, R, S = weight.shape
+        OH, OW = (H - 1) * stride - 2 * pad + R + outpad, (W - 1) * stride - 2 * pad + S + outpad
+    else:
+        stride, pt, pl, pb, pr, _ = geom
+        K, Cw, R, S = weight.shape
+        OH, OW = (H + pt + pb - R) // stride + 1, (W + pl + pr - S) // stride + 1
+    if Cw != C:
+        raise lib.HificError(f"channel mismatch: input {C}, weight {Cw}")
+    return N, C, H, W, K, R, S, OH, OW
+
+
+def _conv_fwd(x, weight, bias, geom, out_f32):
+    cd = ops._cd()
+    if cd == lib.HIFIC_F32 and x.dtype != torch.float32:
+        raise lib.HificError("float32 compute mode needs float32 activations")
+    N, C, H, W, K, R, S, OH, OW = _conv_geom(x, weight, geom)
+    z = torch.empty((N, K, OH, OW), dtype=torch.float32 if cd == lib.HIFIC_F32 or out_f32 else torch.bfloat16, device=x.device)
+    flags = (ops._is_f32(x) | ops._is_f32(z) << 1) if cd == lib.HIFIC_BF16 else 0
+    wsp, wsb = ops._ws(x)
+    if len(geom) == 3:
+        wc = ops._wcache(weight, 0, (N, C, H, W, K, R, S) + geom, cd, flags, None, transposed=True)
+        lib.call("hific_conv_transpose2d_fwd", ptr(x), ptr(weight), ptr(bias), ptr(z), N, C, H, W, K, R, S, *geom, lib.ACT_NONE, cd,
+                 flags, wsp, wsb, *wc, stream())
+    else:
+        wc = ops._wcache(weight, 0, (N, C, H, W, K, R, S) + geom, cd, flags, None)
+        lib.call("hific_conv2d_fwd", ptr(x), ptr(weight), None, ptr(bias), None, ptr(z), N, C, H, W, K, R, S, *geom, lib.ACT_NONE, cd,
+                 flags, wsp, wsb, *wc, stream())
+    return z
+
+
+def _conv_bwd_data(dz, weight, geom, shape, dtype, cd):
+    dx = torch.empty(shape, dtype=dtype, device=dz.device)
+    N, C, H, W, K, R, S, _, _ = _conv_geom(dx, weight, geom)
+    flags = (ops._is_f32(dz) | ops._is_f32(dx) << 1) if cd == lib.HIFIC_BF16 else 0
+    wsp, wsb = ops._ws(dz)
+    wc = ops._wcache(weight, 1, (N, C, H, W, K, R, S) + geom, cd, flags, None, transposed=len(geom) == 3)
+    if len(geom) == 3:
+        lib.call("hific_conv_transpose2d_bwd_data", ptr(dz), ptr(weight), ptr(dx), N, C, H, W, K, R, S, *geom, cd, flags, wsp, wsb, *wc,
+                 stream())
+    else:
+        lib.call("hific_conv2d_bwd_data", ptr(dz), ptr(weight), None, ptr(dx), N, C, H, W, K, R, S, *geom, cd, flags, wsp, wsb, *wc,
+                 stream())
+    return dx
+
+
+def _kept_input(x, q, e, gamma, beta):
+    """What a convolution keeps of its input: the 8-bit form of it, or (no q) the tensor itself."""
+    return (x, None, None, None) if q is None else (q, e, gamma, beta)
+
+
+def _weight_grad(kept, relu, dz, dw, acc, geom, cd):
+    x, e, gamma, beta = kept
+    if e is not None:
+        return _conv_wgrad8(kept, relu, dz, dw, acc, geom, cd)
+    N, C, H, W = x.shape
+    R, S = dw.shape[2], dw.shape[3]
+    K = dz.shape[1]
+    flags = (ops._is_f32(x) | ops._is_f32(dz) << 1) if cd == lib.HIFIC_BF16 else 0
+    if len(geom) == 3:        # (the transposed form's first operand is the input)
+        lib.call("hific_conv_transpose2d_bwd_weight", ptr(x), ptr(dz), ptr(dw), N, C, H, W, K, R, S, *geom, acc, cd, flags, *ops._ws(x),
+                 stream())
+    else:
+        lib.call("hific_conv2d_bwd_weight", ptr(x), ptr(dz), ptr(dw), N, C, H, W, K, R, S, *geom, acc, cd, flags, *ops._ws(x), stream())
+
+
+def _conv_backward(ctx, kept, relu, dz, weight, want_x, want_w, after=None):
+    """Data gradient on the current stream; weight gradient (and `after`) next to it on the side stream where the parameters live in
+    an arena, as ops.ConvNormFn does.  -> dx, dw"""
+    side = want_w and ops._use_side(ctx.w_slot)
+    ev = lib.stream_obj().record_event() if side else None
+    dx = _conv_bwd_data(dz, weight, ctx.geom, ctx.x_shape, ctx.x_dtype, ctx.mode) if want_x else None
+    dw = None
+
+    def params():
+        nonlocal dw
+        if want_w:
+            dwt, acc, dw = ops._grad_target(ctx.w_slot, weight)
+            _weight_grad(kept, relu, dz, dwt, acc, ctx.geom, ctx.mode)
+        if after is not None:
+            after()
+    if side:
+        with ops._SideLaunch(ev, kept[0], kept[1], dz, key=ctx.w_slot):
+            params()
+    else:
+        params()
+    if want_w:
+        ops._written(ctx.w_slot)
+    return dx, dw
+
+
+class ConvNorm8Fn(Function):
+    """ops.ConvNormFn that keeps 8-bit activations: conv (nn.ConvTranspose2d: geom of 3 entries) -> ChannelNorm[+ReLU][+residual].
+    q, e, xg, xb, xrelu: the 8-bit form of x (its weight gradient reads it); without q, x itself is kept."""
+
+    @staticmethod
+    def forward(ctx, x, q, e, xg, xb, xrelu, weight, bias, geom, gamma, beta, eps, relu, resid, code, dt):
+        require_gpu(x, weight, bias, gamma, beta, resid)
+        with _on(x):
+            z = _conv_fwd(x, weight, bias, geom, False)
+            if resid is not None:
+                _like(resid, z, "resid")
+            y, rstd, nq, ne, q2, e2 = _cn8_fwd(z, gamma, beta, resid, eps, relu, _nchw(z), lib.dtype_code(z), code, dt)
+        ctx.geom, ctx.relu, ctx.xrelu, ctx.mode = geom, relu, xrelu, ops._cd()
+        ctx.x_shape, ctx.x_dtype, ctx.has_bias, ctx.has_resid = x.shape, x.dtype, bias is not None, resid is not None
+        ctx.w_slot, ctx.b_slot, ctx.g_slot, ctx.be_slot = (ops._slot(t) for t in (weight, bias, gamma, beta))
+        ctx.save_for_backward(*_kept_input(x, q, e, xg, xb), weight, nq, ne, rstd, gamma, beta)
+        kept = (nq, ne) if resid is None else (q2, e2)
+        ctx.mark_non_differentiable(*kept)
+        ctx.set_materialize_grads(False)
+        return (y,) + kept
+
+    @staticmethod
+    def backward(ctx, dy, _q, _e):
+        _first_order(dy)
+        if dy is None:
+            return (None,) * 16
+        x, e, xg, xb, weight, nq, ne, rstd, gamma, beta = ctx.saved_tensors
+        dy = c16(dy)
+        need = ctx.needs_input_grad
+        with _on(dy):
+            want_n = need[9] or need[10]
+            dgt, acc_g, dg = ops._grad_target(ctx.g_slot, gamma) if want_n else (torch.empty_like(gamma), 0, None)
+            dbt, acc_b, dbe = ops._grad_target(ctx.be_slot, beta) if want_n else (torch.empty_like(beta), 0, None)
+            assert acc_g == acc_b
+            want_b = ctx.has_bias and need[7]
+            dpt, acc_p, db = ops._grad_target(ctx.b_slot, gamma.new_empty(gamma.numel())) if want_b else (None, 0, None)
+            dz = _cn8_bwd(nq, ne, rstd, dy, gamma, beta, ctx.relu, dgt, dbt, acc_g, dpt, acc_p)
+            if want_n:
+                ops._written(ctx.g_slot, ctx.be_slot)
+            if want_b:
+                ops._written(ctx.b_slot)
+            dx, dw = _conv_backward(ctx, (x, e, xg, xb), ctx.xrelu, dz, weight, need[0], need[6])
+        return (dx, None, None, None, None, None, dw, db, None, dg, dbe, None, None, dy if ctx.has_resid else None, None, None)
+
+
+def conv_norm8(x, x8, conv, norm, resid=None, fmt="int8"):
+    """ops.conv_norm with 8-bit checkpoints -> (y, Act8 of y).  `x8`: the Act8 that stands for x (the previous block's, or
+    checkpoint8(x)), or None to keep x itself."""
+    code, dt = _fmt(fmt)
+    if conv.transposed:
+        geom = (conv.stride[0], conv.padding[0], conv.output_padding[0])
+    else:
+        geom = (conv.stride[0],) + tuple(conv.pads) + (conv.hip_pad_mode,)
+    q, e, xg, xb, xrelu = _split8(x8, x)
+    y, q, e = ConvNorm8Fn.apply(c16(x), q, e, xg, xb, xrelu, conv.weight, conv.bias, geom, norm.gamma, norm.beta, _eps(norm.eps),
+                                bool(norm.fuse_relu), None if resid is None else c16(resid), code, dt)
+    if resid is not None:
+        return y, Act8._of(q, e)
+    return y, Act8._of(q, e, norm.gamma.detach(), norm.beta.detach(), bool(norm.fuse_relu))
+
+
+def _split8(x8, x):
+    if x8 is None:
+        return None, None, None, None, False
+    if not isinstance(x8, Act8) or x8.shape != x.shape:
+        raise lib.HificError(f"x8 must be the Act8 of x {tuple(x.shape)}")
+    return x8.q, x8.e, x8.gamma, x8.beta, x8.relu
+
+
+class Conv8Fn(Function):
+    """conv2d whose weight gradient reads the 8-bit form of its input (ops.conv2d with x8=)."""
+
+    @staticmethod
+    def forward(ctx, x, q, e, xg, xb, xrelu, weight, bias, geom, out_f32, bias_grad):
+        require_gpu(x, weight, bias)
+        with _on(x):
+            y = _conv_fwd(x, weight, bias, geom, out_f32)
+        ctx.geom, ctx.xrelu, ctx.mode = geom, xrelu, ops._cd()
+        ctx.x_shape, ctx.x_dtype, ctx.has_bias, ctx.bias_grad = x.shape, x.dtype, bias is not None, bool(bias_grad)
+        ctx.w_slot, ctx.b_slot = ops._slot(weight), ops._slot(bias)
+        ctx.save_for_backward(q, e, xg, xb, weight)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        _first_order(dy)
+        q, e, xg, xb, weight = ctx.saved_tensors
+        dy = c16(dy)
+        need = ctx.needs_input_grad
+        db = None
+        want_b = ctx.has_bias and need[7] and ctx.bias_grad
+
+        def bias():
+            nonlocal db
+            K, plane = dy.shape[1], dy.shape[2] * dy.shape[3]
+            dbt, acc, db = ops._grad_target(ctx.b_slot, weight.new_empty(K))
+            lib.call("hific_channel_sum", ptr(dy), ptr(dbt), dy.shape[0], K, plane, acc, lib.dtype_code(dy), *ops._ws(dy), stream())
+        with _on(dy):
+            dx, dw = _conv_backward(ctx, (q, e, xg, xb), ctx.xrelu, dy, weight, need[0], need[6], bias if want_b else None)
+            if want_b:
+                ops._written(ctx.b_slot)
+        return (dx, None, None, None, None, None, dw, db, None, None, None)
+
+
+def conv2d8(x, x8, weight, bias, geom, out_f32, bias_grad):
+    q, e, xg, xb, xrelu = _split8(x8, x)
+    return Conv8Fn.apply(c16(x), q, e, xg, xb, xrelu, weight, bias, geom, out_f32, bias_grad)
+
+
 # ---- weight gradients of convolutions from an 8-bit input ------------------------------------------------------------------
 # The convolution kernels address one call's tensors with 32-bit element offsets: larger batches go in slices of whole samples
 _MAX_ELEMENTS = 2 ** 31 - 1
@@ -400,33 +627,19 @@ def _slices(N, per_sample):
     return [(i, min(N, i + step)) for i in range(0, N, step)]
 
 
-def _conv_wgrad8(saved, relu, dy, dw, acc, geom):
-    """dw (=|+=) sum dy * pad(x), x the values of `saved` (q, e, gamma, beta) restored to dy's type."""
+def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd):
+    """dw (=|+=) sum dy * pad(x), x the values of `saved` (q, e, gamma, beta) restored to the compute type `cd`; geom of 3 entries:
+    nn.ConvTranspose2d."""
     q, e, gamma, beta = saved
-    stride, pt, pl, pb, pr, pad_mode = geom
     N, C, H, W = q.shape
-    K, R, S = dw.shape[0], dw.shape[2], dw.shape[3]
-    cd = lib.dtype_code(dy)
-    per = max(C * H * W, K * dy.shape[2] * dy.shape[3])
-    for lo, hi in _slices(N, per):
-        x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, dy.dtype)
-        d = c16(dy[lo:hi])
-        lib.call("hific_conv2d_bwd_weight", ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, stride, pt, pl, pb, pr, pad_mode, acc,
-             cd, 0, *ops._ws(x), stream())
-        acc = 1
-
-
-def _convt_wgrad8(saved, relu, dy, dw, acc, geom):
-    q, e, gamma, beta = saved
-    stride, pad, outpad = geom
-    N, C, H, W = q.shape
-    K, R, S = dw.shape[1], dw.shape[2], dw.shape[3]
-    cd = lib.dtype_code(dy)
+    K, R, S = dy.shape[1], dw.shape[2], dw.shape[3]
+    name = "hific_conv_transpose2d_bwd_weight" if len(geom) == 3 else "hific_conv2d_bwd_weight"
+    xt = torch.float32 if cd == lib.HIFIC_F32 else torch.bfloat16
+    flags = ops._is_f32(dy) << 1 if cd == lib.HIFIC_BF16 else 0
     for lo, hi in _slices(N, max(C * H * W, K * dy.shape[2] * dy.shape[3])):
-        x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, dy.dtype)
+        x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, xt)
         d = c16(dy[lo:hi])
-        lib.call("hific_conv_transpose2d_bwd_weight", ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, stride, pad, outpad, acc,
-             cd, 0, *ops._ws(x), stream())
+        lib.call(name, ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, *geom, acc, cd, flags, *ops._ws(x), stream())
         acc = 1
 
 
@@ -462,7 +675,7 @@ def conv2d_weight_grad8(a, dy, kernel, stride=1, pads=(0, 0, 0, 0), pad_mode=lib
     if N == 0:
         return dw.zero_()
     with _on(dy):
-        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pt, pl, pb, pr, pad_mode))
+        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pt, pl, pb, pr, pad_mode), lib.dtype_code(dy))
     return dw
 
 
@@ -480,5 +693,5 @@ def conv_transpose2d_weight_grad8(a, dy, kernel, stride, pad, outpad):
     if N == 0:
         return dw.zero_()
     with _on(dy):
-        _convt_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pad, outpad))
+        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pad, outpad), lib.dtype_code(dy))
     return dw

@@ -112,7 +112,29 @@ class Encoder(nn.Module):
             planes.append((conv.out_channels, H, W))
         return planes
 
+    def _forward_checkpoint8(self, x, fmt):
+        """The plain chain whose backward pass keeps 8-bit activations (ops.set_checkpoint8); the image itself is kept as it is."""
+        from .. import ops
+        x8 = None
+        for blk in (self.conv_block1, self.conv_block2, self.conv_block3, self.conv_block4, self.conv_block5):
+            x, x8 = ops.conv_norm8(x, x8, blk[1], blk[2], fmt=fmt)
+        out = self.conv_block_out[1]
+        return ops.conv2d(x, out.weight, out.bias, stride=out.stride[0], pads=out.pads, pad_mode=out.hip_pad_mode, out_f32=True, x8=x8)
+
+    def _checkpoint8_fmt(self, x):
+        from .. import ops
+        import torch
+        fmt = ops.checkpoint8_fmt()
+        blk = self.conv_block1
+        ok = fmt is not None and torch.is_grad_enabled() and x.is_cuda and isinstance(blk[2], channel.ChannelNorm2D) \
+            and blk[1].bias_grad_in_norm and not (ops.exact_index_on() and ops.get_compute_dtype() == torch.bfloat16
+                                                  and blk[1].exact_index_chain)
+        return fmt if ok else None
+
     def _forward_plain(self, x):
+        fmt = self._checkpoint8_fmt(x)
+        if fmt is not None:
+            return self._forward_checkpoint8(x, fmt)
         x = self.conv_block1(x)
         x = self.conv_block2(x)
         x = self.conv_block3(x)

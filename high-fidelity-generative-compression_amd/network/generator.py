@@ -169,12 +169,35 @@ class Generator(nn.Module):
             h = cn(h, u[0], u[1])
         return self.conv_block_out(h)
 
+    def _forward_checkpoint8(self, x, fmt):
+        """_forward_plain_fused whose backward pass keeps 8-bit activations (ops.set_checkpoint8): every block hands the next one
+        its output and the 8-bit form of it."""
+        cn = ops.conv_norm8
+        h = self.conv_block_init[0](x)
+        head, h8 = cn(h, ops.checkpoint8(h, fmt), self.conv_block_init[2], self.conv_block_init[3], fmt=fmt)
+        h, head_skip = ops.fork(head)
+        for m in range(self.n_residual_blocks):
+            blk = getattr(self, f'resblock_{m}')
+            h_conv, h_id = ops.fork(h)
+            r, r8 = cn(h_conv, h8, blk.conv1, blk.norm1, fmt=fmt)
+            h, h8 = cn(r, r8, blk.conv2, blk.norm2, resid=h_id, fmt=fmt)
+        h = ops.add(h, head_skip)
+        h8 = ops.checkpoint8(h, fmt)
+        for i in range(4):
+            u = getattr(self, f'upconv_block{i + 1}')
+            h, h8 = cn(h, h8, u[0], u[1], fmt=fmt)
+        out = self.conv_block_out[1]
+        return ops.conv2d(h, out.weight, out.bias, stride=1, pads=out.pads, pad_mode=out.hip_pad_mode, x8=h8)
+
     def forward(self, x):
         if self._exact_chain_ok(x):
             return self._forward_exact_chain(x)
         exact_unfused = self.conv_block_out[1].exact_recon and (
             ops.exact_training_on() or (ops.exact_reconstruction_on() and not torch.is_grad_enabled()))
         if not exact_unfused and self._plain_fused_ok(x):
+            fmt = ops.checkpoint8_fmt()
+            if fmt is not None and torch.is_grad_enabled():
+                return self._forward_checkpoint8(x, fmt)
             return self._forward_plain_fused(x)
         head = self.conv_block_init(x)
         if self.sample_noise is True:

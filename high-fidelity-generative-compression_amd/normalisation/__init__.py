@@ -1,1 +1,1 @@
-from . import channel, instance  # noqa: F401
+from . import channel, instance, rms  # noqa: F401

@@ -874,11 +874,16 @@ class Conv2dFn(Function):
 
 
 def conv2d(x, weight, bias, stride=1, pads=(0, 0, 0, 0), pad_mode=lib.PAD_ZERO, act=None, out_f32=False, w_scale=None,
-           exact=False, bias_grad=True, x3=None):
-    """`exact=True` (bf16 compute mode only): split-bf16 forward on float32 activations, float32 output - the exact-index
+           exact=False, bias_grad=True, x3=None, x8=None):
+    """`x8`: the Act8 that stands for `x` (channel_norm8, checkpoint8): the backward pass keeps it in the place of `x` (plain
+    convolutions without an activation).  `exact=True` (bf16 compute mode only): split-bf16 forward on float32 activations, float32 output - the exact-index
     chain (see set_exact_index); the backward pass is the ordinary bf16 one.  `x3`: the (hi, lo, hi) image of `x` when the
     caller already has it (then `x` may be the nominal bf16 activation)."""
     pt, pl, pb, pr = pads
+    if x8 is not None:
+        if exact or w_scale is not None or act not in (None, "none"):
+            raise lib.HificError("conv2d(x8=): only a plain convolution without activation reads an 8-bit input")
+        return conv2d8(x, x8, weight, bias, (stride, pt, pl, pb, pr, pad_mode), out_f32, bias_grad)
     if exact and x3 is None and _compute_dtype == torch.bfloat16 and x.dtype != torch.float32:
         x = cast_grad(x, torch.float32)
     return Conv2dFn.apply(_c16(x), weight, bias, (stride, pt, pl, pb, pr, pad_mode), act, out_f32, w_scale, exact,
@@ -2120,4 +2125,4 @@ def hyper_symbols_and_indices(hyperlatents):
 # ------------------------------------------------------------------------------------------------------
 # activations in 8 bits, the norms that write and read them, root-mean-square norm (act8.py)
 from .act8 import (Act8, checkpoint8, restore8, rms_norm, rms_norm8, channel_norm8, channel_norm_grad8,  # noqa: E402,F401
-                   conv2d_weight_grad8, conv_transpose2d_weight_grad8)
+                   conv2d_weight_grad8, conv_transpose2d_weight_grad8, conv_norm8, conv2d8, set_checkpoint8, checkpoint8_fmt)
