@@ -627,6 +627,12 @@ def _slices(N, per_sample):
     return [(i, min(N, i + step)) for i in range(0, N, step)]
 
 
+@functools.lru_cache(maxsize=1024)
+def _wgrad8_ws_bytes(*shape):
+    """Workspace of the kernel that reads the 8-bit tensor itself; 0 where restoring it for the natural-order kernels is faster."""
+    return int(lib.raw("hific_wgrad8_ws_bytes")(*shape[:10])) if lib.raw("hific_wgrad8_prefer")(*shape) else 0
+
+
 def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd):
     """dw (=|+=) sum dy * pad(x), x the values of `saved` (q, e, gamma, beta) restored to the compute type `cd`; geom of 3 entries:
     nn.ConvTranspose2d."""
@@ -636,9 +642,18 @@ def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd):
     name = "hific_conv_transpose2d_bwd_weight" if len(geom) == 3 else "hific_conv2d_bwd_weight"
     xt = torch.float32 if cd == lib.HIFIC_F32 else torch.bfloat16
     flags = ops._is_f32(dy) << 1 if cd == lib.HIFIC_BF16 else 0
-    for lo, hi in _slices(N, max(C * H * W, K * dy.shape[2] * dy.shape[3])):
-        x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, xt)
+    tr, OH, OW = int(len(geom) == 3), dy.shape[2], dy.shape[3]
+    for lo, hi in _slices(N, max(C * H * W, K * OH * OW)):
         d = c16(dy[lo:hi])
+        n = _wgrad8_ws_bytes(tr, hi - lo, C, H, W, K, R, S, OH, OW, geom[0]) if dy.dtype == torch.bfloat16 and cd == lib.HIFIC_BF16 else 0
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
+            pt, pl, mode = (geom[1], geom[1], lib.PAD_ZERO) if tr else (geom[1], geom[2], geom[5])
+            lib.call("hific_wgrad8", tr, ptr(q[lo:hi]), ptr(e[lo:hi]), _CODE[q.dtype], ptr(gamma), ptr(beta), int(relu), ptr(d), ptr(dw),
+                     hi - lo, C, H, W, K, R, S, OH, OW, geom[0], pt, pl, mode, acc, ptr(ws), n, stream())
+            acc = 1
+            continue
+        x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, xt)
         lib.call(name, ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, *geom, acc, cd, flags, *ops._ws(x), stream())
         acc = 1
 

@@ -9,7 +9,7 @@ mkdir -p $OBJDIR
 # no packed-float32 instructions (v_pk_add/mul/fma_f32): some of their forms have given wrong results on this hardware now and
 # then; scalar float code has the same results and the same rate per element
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA"
-SRCS="gconv gconv_mpvc gconv_sp9 gconv_pack gconv_wgrad gconv_wgrad_nat gconv_wgrad_c3 gconv_pl gconv_wr elementwise norm norm8 act8 entropy lpips augment capi"
+SRCS="gconv gconv_mpvc gconv_sp9 gconv_pack gconv_wgrad gconv_wgrad_nat gconv_wgrad_c3 gconv_pl gconv_wr elementwise norm norm8 act8 wgrad8 entropy lpips augment capi"
 OBJS=""
 PIDS=""
 NAMES=""

@@ -133,6 +133,23 @@ def test_entry_points_refuse_bad_arguments(hific):
     cnb = lib.raw("hific_channelnorm8_bwd")
     assert cnb(p, p, 0, p, p, p, p, p, p, p, 0, None, 0, 1, 8, 4, 0, 0, p, 4, None) == -2
     assert lib.raw("hific_norm8_bwd_ws_bytes")(0, 8, 4) == 0
+    wg = lib.raw("hific_wgrad8")
+    need = lib.raw("hific_wgrad8_ws_bytes")(0, 2, 8, 6, 6, 4, 3, 3, 6, 6)
+    assert need > 0 and lib.raw("hific_wgrad8_ws_bytes")(0, 2, 8, 6, 6, 0, 3, 3, 6, 6) == 0
+    ok = [0, p, p, 0, None, None, 0, p, p, 2, 8, 6, 6, 4, 3, 3, 6, 6, 1, 1, 1, 1, 0, p, need, None]
+
+    def refuse(at, value):
+        args = list(ok)
+        args[at] = value
+        return wg(*args)
+    assert refuse(1, None) == refuse(3, 5) == refuse(4, p) == refuse(6, 1) == refuse(9, 0) == refuse(18, 0) == refuse(21, 3) == -1
+    assert refuse(19, 6) == -1                                             # a reflection pad as large as the plane
+    assert refuse(16, 99) == -1                                            # positions past the second border
+    assert refuse(0, 1) == -1                                              # no reflection for the transposed form
+    assert refuse(24, need - 1) == -2 and refuse(23, ctypes.c_void_p(4097)) == -2
+    pref = lib.raw("hific_wgrad8_prefer")
+    assert pref(0, 2, 120, 61, 47, 240, 3, 3, 31, 24, 2) == 1 and pref(0, 16, 960, 16, 16, 960, 3, 3, 16, 16, 1) == 0
+    assert pref(0, 0, 120, 61, 47, 240, 3, 3, 31, 24, 2) == 0
 
 
 def test_large_batches_go_in_slices(hific):
