@@ -175,10 +175,11 @@ __device__ __forceinline__ void q8_scales(u32x2_t e, float* scale, float* s128) 
 }
 
 // eight normalised values of a channel whose ReLU follows, as x = xh / scale, v = fma(gs, x, beta) with gs = gamma * scale (the
-// same product as gamma * xh): q8_round_masked of each.  No clamp: max|xh| gave the exponent, so |x| <= QMAX, and the neighbour
+// same product as gamma * xh): q8_round_masked of each, and v
+// becomes relu(v).  No clamp: max|xh| gave the exponent, so |x| <= QMAX, and the neighbour
 // that is taken lies between x and the nearest value's other side.
 template <int FMT>
-__device__ __forceinline__ u32x2_t q8_pack8_masked(const float* x, const float* v, const float* gs, float beta, float gamma) {
+__device__ __forceinline__ u32x2_t q8_pack8_masked(const float* x, float* v, const float* gs, float beta, float gamma) {
     const float up = gamma > 0.f ? 1.f : -1.f;                   // the step towards the ReLU's open side
     if (FMT == HIFIC_Q_INT8) {
         float t[8];
@@ -188,6 +189,7 @@ __device__ __forceinline__ u32x2_t q8_pack8_masked(const float* x, const float* 
             const bool on = relu_on(v[j]);
             const float other = n + (on ? up : -up);
             t[j] = relu_on(fmaf(gs[j], n, beta)) != on ? other : n;
+            v[j] = on ? v[j] : 0.f;
         }
         return q8_pack8<FMT, false>(t);
     }
@@ -203,6 +205,7 @@ __device__ __forceinline__ u32x2_t q8_pack8_masked(const float* x, const float* 
                 const unsigned c = q8_next<FMT>((q[h] >> (8 * j)) & 0xffu, (on ? up : -up) > 0.f);
                 q[h] = (q[h] & ~(0xffu << (8 * j))) | (c << (8 * j));
             }
+            v[4 * h + j] = on ? v[4 * h + j] : 0.f;
         }
     }
     return q;
@@ -213,34 +216,50 @@ template <typename T> __device__ __forceinline__ T* at(T* base, unsigned bytes) 
 template <typename T> __device__ __forceinline__ const T* at(const T* base, unsigned bytes) { return (const T*)((const char*)base + bytes); }
 
 // Planes: lane = (group of eight positions pl = lane % LPX, channel sub-group lane / LPX).  v[j], this lane's partial of position j,
-// is combined over the 64 / LPX sub-groups of the wave: up to three steps exchange halves (4 + 2 + 1 shuffles where eight separate
-// butterflies would take 8 per step), further ones carry one value.  out[pl * 8 + j] receives the wave's result.
-template <int LPX, bool MAX>
-__device__ __forceinline__ unsigned tile_op(unsigned x, unsigned y) { return MAX ? umax(x, y) : x + y; }
-template <int LPX, bool MAX>
-__device__ __forceinline__ float tile_op(float x, float y) { return MAX ? fmaxf(x, y) : x + y; }
+// is combined over the 64 / LPX sub-groups of the wave; out[pl * 8 + j] receives the wave's result.
+// Every step halves what a lane carries: the lanes of one half keep the first values, those of the other the last ones.  Across
+// 32 and 16 lanes that is one swap instruction and one operation per value that is kept, no select and no address (the swap gives
+// {x of the low lanes, y of the low lanes} and {x of the high, y of the high}); across 8 lanes a rotation of the row; what is left
+// (LPX < 8) is one value.  Eight values over 4 sub-groups: 12 instructions, where shuffles with selects took about 90 and the two
+// or three reductions of a tile more than the arithmetic of its values.
+template <bool MAX> __device__ __forceinline__ unsigned tile_op(unsigned x, unsigned y) { return MAX ? umax(x, y) : x + y; }
+template <bool MAX> __device__ __forceinline__ float tile_op(float x, float y) { return MAX ? fmaxf(x, y) : x + y; }
+template <bool MAX, typename V>
+__device__ __forceinline__ V tile_swap32(V x, V y) {
+    const u32x2_t r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+    return tile_op<MAX>(__builtin_bit_cast(V, (unsigned)r[0]), __builtin_bit_cast(V, (unsigned)r[1]));
+}
+template <bool MAX, typename V>
+__device__ __forceinline__ V tile_swap16(V x, V y) {
+    const u32x2_t r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+    return tile_op<MAX>(__builtin_bit_cast(V, (unsigned)r[0]), __builtin_bit_cast(V, (unsigned)r[1]));
+}
+template <int CTRL, typename V>                                  // a data-parallel-primitive move within rows of 16 lanes
+__device__ __forceinline__ V tile_dpp(V x) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
 template <int LPX, bool MAX, typename V>
 __device__ __forceinline__ void tile_reduce(const V* v, V* out) {
-    constexpr int SUBS = 64 / LPX, KEEP = SUBS >= 8 ? 1 : 8 / SUBS;      // values per lane at the end
-    const int lane = threadIdx.x & 63, sub = lane / LPX;
-    auto shfl = [](V x, int o) { return __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(int, x), o, 64)); };
+    const int lane = threadIdx.x & 63;
     V a[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = v[j];
-    int first = 0;
+    for (int j = 0; j < 4; ++j) a[j] = tile_swap32<MAX>(v[j], v[4 + j]);
+    int first = (lane & 32) ? 4 : 0;
+    if constexpr (LPX <= 16) {
 #pragma unroll
-    for (int s = 0; s < 3; ++s) {
-        if ((1 << s) >= SUBS) break;
-        const int half = 4 >> s;
-        const bool hi = (sub >> s) & 1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < half) a[j] = tile_op<LPX, MAX>(hi ? a[half + j] : a[j], shfl(hi ? a[j] : a[half + j], LPX << s));
-        first += hi ? half : 0;
+        for (int j = 0; j < 2; ++j) a[j] = tile_swap16<MAX>(a[j], a[2 + j]);
+        first += (lane & 16) ? 2 : 0;
     }
-#pragma unroll
-    for (int o = 8 * LPX; o < 64; o <<= 1) a[0] = tile_op<LPX, MAX>(a[0], shfl(a[0], o));
-    if (sub < 8)
+    if constexpr (LPX <= 8) {
+        const bool hi = lane & 8;
+        a[0] = tile_op<MAX>(hi ? a[1] : a[0], tile_dpp<0x128>(hi ? a[0] : a[1]));       // row_ror:8 = the lane 8 further
+        first += hi ? 1 : 0;
+    }
+    if constexpr (LPX <= 4) a[0] = tile_op<MAX>(a[0], __builtin_bit_cast(V, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, a[0]), 0x101f)));  // lane ^ 4
+    if constexpr (LPX <= 2) a[0] = tile_op<MAX>(a[0], tile_dpp<0x4e>(a[0]));            // quad_perm 2 3 0 1
+    if constexpr (LPX <= 1) a[0] = tile_op<MAX>(a[0], tile_dpp<0xb1>(a[0]));            // quad_perm 1 0 3 2
+    constexpr int KEEP = LPX == 32 ? 4 : (LPX == 16 ? 2 : 1);
+    if (LPX >= 8 || (lane & 7) < LPX)
 #pragma unroll
         for (int j = 0; j < KEEP; ++j) out[(lane % LPX) * 8 + first + j] = a[j];
 }

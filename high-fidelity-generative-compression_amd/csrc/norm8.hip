@@ -173,13 +173,10 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
                 for (int j = 0; j < 8; ++j) acc[j] += xr[k].get(j);
         tile_reduce<LPX, false>(acc, red[wave]);
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = pl * 8 + j;
-            mu[j] = ((red[0][i] + red[1][i]) + (red[2][i] + red[3][i])) * p.rc;
-            acc[j] = 0.f;
-        }
+        if (tid < TP) st_r[tid] = ((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) * p.rc;
         __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { mu[j] = st_r[pl * 8 + j]; acc[j] = 0.f; }
     }
     // each pass unpacks again: kept unpacked, the values would take twice the registers
 #pragma unroll
@@ -215,7 +212,13 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
     // x = d * (r / scale) is xh / scale: dividing by a power of two commutes with the rounding, and so does gs below
     float r[8], ri[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { r[j] = st_r[pl * 8 + j]; ri[j] = FMT != Q_NONE ? r[j] * st_inv[pl * 8 + j] : 0.f; am[j] = 0.f; }
+    for (int j = 0; j < 8; ++j) {
+        const float inv = FMT != Q_NONE ? st_inv[pl * 8 + j] : 0.f;
+        r[j] = st_r[pl * 8 + j]; ri[j] = r[j] * inv; am[j] = 0.f;
+        // behind a ReLU only x and gs are formed: r's place holds the scale 1 / inv, a power of two (2^127 for a token that is not
+        // finite: its values are NaN)
+        if (MODE == M_CHAN && FMT != Q_NONE && p.relu) r[j] = __uint_as_float(0x7f000000u - __float_as_uint(inv));
+    }
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
         const int c = g + G * k;
@@ -225,8 +228,7 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
             float x[8], gs[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                // 1 / inv, a power of two (2^127 for a token that is not finite: its values are NaN)
-                gs[j] = w[k] * __uint_as_float(0x7f000000u - __float_as_uint(st_inv[pl * 8 + j]));
+                gs[j] = w[k] * r[j];
                 x[j] = (xr[k].get(j) - mu[j]) * ri[j];
                 o[j] = fmaf(gs[j], x[j], b[MODE == M_CHAN ? k : 0]);
             }
@@ -248,9 +250,6 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
             }
         }
         if constexpr (MODE == M_CHAN) {
-            if (p.relu)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = relu_nan(o[j]);
             if (p.resid) {               // both terms rounded to the storage type first, as norm and add one after the other
                 V8<T> t; t.set(o);
 #pragma unroll
@@ -431,7 +430,7 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
 template <typename T, int MODE, int SRC, int LPX, int CPT>
 __global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
     constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
-    __shared__ float red[2][4][TP];
+    __shared__ float red[2][4][TP], st[2][TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
     const unsigned per = (p.tiles + pit - 1) / pit;                  // workgroups per image
     const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / per, t0 = (bid - n * per) * pit;
@@ -498,16 +497,16 @@ __global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p,
         if constexpr (CPT > 2)
 #pragma unroll
         for (int k = 0; k < CPT; ++k) { dy[k].forget(); if constexpr (SRC == SRC_T) hr[k].forget(); else forget(q[k]); }
-        if (it > 0) __syncthreads();                                 // the readers of the previous tile's sums are done
         tile_reduce<LPX, false>(s2, red[1][wave]);
         if (MODE == M_CHAN) tile_reduce<LPX, false>(s1, red[0][wave]);
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = pl * 8 + j;
-            s2[j] = ((red[1][0][i] + red[1][1][i]) + (red[1][2][i] + red[1][3][i])) * p.rv;
-            if (MODE == M_CHAN) s1[j] = ((red[0][0][i] + red[0][1][i]) + (red[0][2][i] + red[0][3][i])) * p.rc;
+        if (tid < TP) {
+            st[1][tid] = ((red[1][0][tid] + red[1][1][tid]) + (red[1][2][tid] + red[1][3][tid])) * p.rv;
+            if (MODE == M_CHAN) st[0][tid] = ((red[0][0][tid] + red[0][1][tid]) + (red[0][2][tid] + red[0][3][tid])) * p.rc;
         }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s2[j] = st[1][pl * 8 + j]; if (MODE == M_CHAN) s1[j] = st[0][pl * 8 + j]; }
 #pragma unroll
         for (int k = 0; k < CPT; ++k) {
             const int c = g + G * k;
