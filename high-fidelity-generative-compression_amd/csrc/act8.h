@@ -297,7 +297,7 @@ static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
         else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F); } else { TILE_CPT(1, t, MOST, F); }                             \
     } while (0)
 #define TILE_CPT(LPX, t, MOST, F)                                                                                         \
-    if ((t).cpt <= 1) F(LPX, 1); else if ((t).cpt <= 2) F(LPX, 2); else if ((t).cpt <= 4) F(LPX, 4); else F(LPX, ((MOST) < 8 ? 4 : 8))
+    if ((t).cpt <= 1) { F(LPX, 1); } else if ((t).cpt <= 2) { F(LPX, 2); } else if ((t).cpt <= 4) { F(LPX, 4); } else { F(LPX, ((MOST) < 8 ? 4 : 8)); }
 
 // Rows: L lanes and K groups of eight channels per lane hold a row.  Sums and maxima over the row's L lanes, through LDS where a
 // row has the whole workgroup.

@@ -9,12 +9,12 @@ mkdir -p $OBJDIR
 # no packed-float32 instructions (v_pk_add/mul/fma_f32): some of their forms have given wrong results on this hardware now and
 # then; scalar float code has the same results and the same rate per element
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops $EXTRA"
-SRCS="gconv gconv_mpvc gconv_sp9 gconv_pack gconv_wgrad gconv_wgrad_nat gconv_wgrad_c3 gconv_pl gconv_wr elementwise norm norm8 act8 wgrad8 entropy lpips augment capi"
+SRCS="gconv gconv_mpvc gconv_sp9 gconv_pack gconv_wgrad gconv_wgrad_nat gconv_wgrad_c3 gconv_pl gconv_wr elementwise norm norm8_fwd norm8_bwd act8 wgrad8 entropy lpips augment capi"
 OBJS=""
 PIDS=""
 NAMES=""
 for f in $SRCS; do
-  if [ ! -f $OBJDIR/$f.o ] || [ build.sh -nt $OBJDIR/$f.o ] || [ $f.hip -nt $OBJDIR/$f.o ] || [ common.h -nt $OBJDIR/$f.o ] || [ act8.h -nt $OBJDIR/$f.o ] || [ gconv.h -nt $OBJDIR/$f.o ] || [ gconv_dev.h -nt $OBJDIR/$f.o ] || [ gconv_stage.h -nt $OBJDIR/$f.o ]; then
+  if [ ! -f $OBJDIR/$f.o ] || [ build.sh -nt $OBJDIR/$f.o ] || [ $f.hip -nt $OBJDIR/$f.o ] || [ common.h -nt $OBJDIR/$f.o ] || [ act8.h -nt $OBJDIR/$f.o ] || [ norm8.h -nt $OBJDIR/$f.o ] || [ gconv.h -nt $OBJDIR/$f.o ] || [ gconv_dev.h -nt $OBJDIR/$f.o ] || [ gconv_stage.h -nt $OBJDIR/$f.o ]; then
     rm -f $OBJDIR/$f.o                            # a failed compile must never leave a stale object to link
     hipcc $FLAGS -c $f.hip -o $OBJDIR/$f.o &
     PIDS="$PIDS $!"
