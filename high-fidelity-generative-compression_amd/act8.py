@@ -19,6 +19,7 @@ from .lib import ptr, stream, require_gpu
 FORMATS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _INF = float("inf")
+_INT = 2 ** 31 - 1
 
 
 def _fmt(fmt):
@@ -32,10 +33,12 @@ def _nchw(x, name="x"):
     d = x.dim()
     if d < 2 or x.size(1) < 1:
         raise lib.HificError(f"{name} must be [N, C, ...] with at least one channel, got {tuple(x.shape)}")
-    hw = 1
+    n, c, hw = x.size(0), x.size(1), 1
     for i in range(2, d):
         hw *= x.size(i)
-    return x.size(0), x.size(1), hw
+    if n > _INT or c > _INT or hw > _INT:
+        raise lib.HificError(f"{name}: a dimension of {tuple(x.shape)} is beyond 32 bits")
+    return n, c, hw
 
 
 def _tokens(x):
@@ -358,9 +361,9 @@ def _norm_args(x, gamma, beta, name):
 
 def channel_norm8(x, gamma, beta, eps=1e-3, relu=False, resid=None, fmt="int8"):
     """channel_norm (src/normalisation/channel.py:48-59, with the ReLU or the residual behind it) -> (y, Act8): y as channel_norm
-    gives it, and the Act8 stands for y too - what the next convolution's weight gradient reads (conv2d(x8=)).  The backward pass
-    of the norm keeps its normalised input in 8 bits and nothing else of x or y.  With `relu` the kept values are on the same
-    side of the ReLU as the forward values."""
+    gives it (but for a position with an infinity or NaN, which stays NaN behind the ReLU too), and the Act8 stands for y too -
+    what the next convolution's weight gradient reads (conv2d(x8=)).  The backward pass of the norm keeps its normalised input in
+    8 bits and nothing else of x or y.  With `relu` the kept values are on the same side of the ReLU as the forward values."""
     geom = _norm_args(x, gamma, beta, "channel_norm8")
     code, dt = _fmt(fmt)
     cd = lib.dtype_code(x)
@@ -633,7 +636,20 @@ def _wgrad8_ws_bytes(*shape):
     return int(lib.raw("hific_wgrad8_ws_bytes")(*shape[:10])) if lib.raw("hific_wgrad8_prefer")(*shape) else 0
 
 
-def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd):
+def _graph_ws(x, tr, geom, N, C, H, W, K, R, S, cd):
+    """Workspace of the restored form: the stream's, or inside a graph capture one of the graph's own (two graphs captured on one
+    stream may replay on two)."""
+    if not torch.cuda.is_current_stream_capturing():
+        return ops._ws(x)
+    if tr:
+        n = lib.raw("hific_conv_transpose2d_ws_bytes")(N, C, H, W, K, R, S, *geom, cd)
+    else:
+        n = lib.raw("hific_conv2d_ws_bytes")(N, C, H, W, K, R, S, *geom[:5], cd)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    return ws.data_ptr(), n
+
+
+def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd, own_ws=False):
     """dw (=|+=) sum dy * pad(x), x the values of `saved` (q, e, gamma, beta) restored to the compute type `cd`; geom of 3 entries:
     nn.ConvTranspose2d."""
     q, e, gamma, beta = saved
@@ -654,7 +670,8 @@ def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd):
             acc = 1
             continue
         x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, xt)
-        lib.call(name, ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, *geom, acc, cd, flags, *ops._ws(x), stream())
+        ws = _graph_ws(x, tr, geom, hi - lo, C, H, W, K, R, S, cd) if own_ws else ops._ws(x)
+        lib.call(name, ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, *geom, acc, cd, flags, *ws, stream())
         acc = 1
 
 
@@ -690,7 +707,7 @@ def conv2d_weight_grad8(a, dy, kernel, stride=1, pads=(0, 0, 0, 0), pad_mode=lib
     if N == 0:
         return dw.zero_()
     with _on(dy):
-        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pt, pl, pb, pr, pad_mode), lib.dtype_code(dy))
+        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pt, pl, pb, pr, pad_mode), lib.dtype_code(dy), True)
     return dw
 
 
@@ -708,5 +725,5 @@ def conv_transpose2d_weight_grad8(a, dy, kernel, stride, pad, outpad):
     if N == 0:
         return dw.zero_()
     with _on(dy):
-        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pad, outpad), lib.dtype_code(dy))
+        _conv_wgrad8(a.tensors(), a.relu, dy, dw, 0, (stride, pad, outpad), lib.dtype_code(dy), True)
     return dw

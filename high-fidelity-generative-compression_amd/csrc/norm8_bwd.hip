@@ -79,18 +79,16 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
     }
 }
 
-// Planes: as norm8_fwd_tile_kernel.  A workgroup takes `pit` tiles of one image in turn and keeps the sums of its channels in
-// registers: part[workgroup][0..2][c] as norm8_param_kernel.
+// Planes: as norm8_fwd_tile_kernel.  A workgroup takes `pit` tiles in turn (p.tokens counts tiles here) and keeps the sums of its
+// channels in registers: part[workgroup][0..2][c] as norm8_param_kernel.
 template <typename T, int MODE, int SRC, int LPX, int CPT>
 __global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
     constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
     __shared__ float red[2][4][TP], st[2][TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
-    const unsigned per = (p.tiles + pit - 1) / pit;                  // workgroups per image
-    const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / per, t0 = (bid - n * per) * pit;
+    const unsigned bid = xcd_block(blockIdx.x, blocks);
     const unsigned octs = ((unsigned)p.HW + 7) >> 3;
     const unsigned kst = (unsigned)G * p.HW;                         // channel k of this lane: img + off + k * kst
-    const size_t img = (size_t)n * p.C * p.HW;
     float w[CPT], b[MODE == M_CHAN ? CPT : 1], pg[CPT], pb[MODE == M_CHAN ? CPT : 1], pd[MODE == M_CHAN ? CPT : 1];
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
@@ -98,8 +96,11 @@ __global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p,
         w[k] = p.w[ci]; pg[k] = 0.f;
         if constexpr (MODE == M_CHAN) { b[k] = p.b[ci]; pb[k] = 0.f; pd[k] = 0.f; }
     }
-    for (unsigned it = 0; it < pit && t0 + it < p.tiles; ++it) {
-        const unsigned oct = (t0 + it) * LPX + pl;
+    for (unsigned it = 0; it < pit; ++it) {
+        const long long lin = (long long)bid * pit + it;             // tile of the batch: small planes share a workgroup
+        if (lin >= p.tokens) break;
+        const unsigned n = (unsigned)(lin / p.tiles), oct = (unsigned)(lin - (long long)n * p.tiles) * LPX + pl;
+        const size_t img = (size_t)n * p.C * p.HW;
         const bool ok = oct < octs;
         const unsigned hw0 = umin(ok ? oct * 8 : 0u, (unsigned)p.HW - 8);
         const int dup = ok ? (int)(oct * 8 - hw0) : 8;               // values that another lane adds to the channels' sums
@@ -334,16 +335,13 @@ int norm8_nsplit(int N, int C, int HW) {                             // ~1024 wo
 }
 // tiles per workgroup of the backward plane kernel: 512 workgroups, two per CU (what its registers allow), each with its share of
 // the tiles - one round, few rows of channel sums (16x120x128x128: 43 us, with 1024 workgroups 47.5, with 2048 53)
-unsigned norm8_pit(const TileCfg& t, long long N) {
-    unsigned pit = (unsigned)(t.blocks / 512);
-    return pit < 1 ? 1 : (pit > t.tiles ? t.tiles : pit);
-}
+unsigned norm8_pit(const TileCfg& t) { return (unsigned)(t.blocks < 512 ? 1 : cdivl(t.blocks, 512)); }
 // rows of channel sums that the backward pass writes
 template <typename T>
 size_t norm8_rows(int mode, int N, int C, int HW) {
     if (HW >= 8) {
         const TileCfg t = tile_pick(N, C, HW, tile_most<T>());
-        if (t.lpx) return (size_t)cdiv((int)t.tiles, (int)norm8_pit(t, N)) * N;
+        if (t.lpx) return (size_t)cdivl(t.blocks, norm8_pit(t));
     }
     if (mode == M_RMS && HW == 1 && C >= 8) {
         const RowCfg r = row_pick(N, C);
@@ -366,7 +364,8 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
     if (rows > 0x7fffffffull) return HIFIC_ERR_UNSUPPORTED;
     if (t.lpx) {
         p.tiles = t.tiles;
-        const unsigned pit = norm8_pit(t, N);
+        const unsigned pit = norm8_pit(t);
+        p.tokens = t.blocks;
 #define BWD(LPX, CPT) hipLaunchKernelGGL((norm8_bwd_tile_kernel<T, MODE, SRC, LPX, CPT>), dim3((unsigned)rows), dim3(256), 0, st, p, (unsigned)rows, pit)
         TILE_DISPATCH(t, tile_most<T>(), BWD);
 #undef BWD

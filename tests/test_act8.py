@@ -98,7 +98,7 @@ def test_arguments_are_checked_before_the_device(hific):
            lambda: ops.Act8(torch.zeros(2, 8), torch.zeros(2, dtype=torch.uint8)),
            lambda: ops.Act8(torch.zeros(2, 8, dtype=torch.int8), torch.zeros(3, dtype=torch.uint8)),
            lambda: ops.Act8(torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2, dtype=torch.uint8), relu=True),
-           lambda: ops.channel_norm_grad8(x, x, w, w, w), lambda: ops.conv2d_weight_grad8(x, x, (3, 3))]
+           lambda: ops.checkpoint8(torch.empty(1, 1, 1).expand(1, 1, 2 ** 31)), lambda: ops.channel_norm_grad8(x, x, w, w, w), lambda: ops.conv2d_weight_grad8(x, x, (3, 3))]
     for f in bad:
         with pytest.raises(lib.HificError):
             f()

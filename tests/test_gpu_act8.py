@@ -297,6 +297,24 @@ def test_channel_norm8(hific, dev, shape, dt, relu, resid, fmt):
     assert torch.equal(dx, grads[0]) and torch.equal(dg, grads[1]) and torch.equal(db, grads[2])
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("shape", [(2, 64, 8, 8), (3, 60, 24, 40), (2, 33, 5, 7), (3, 47, 2, 3), (40, 96)])
+def test_masks_agree_forward_and_backward_for_any_gamma(hific, dev, shape, fmt):
+    """gamma of both signs, zero and tiny: a position passes gradient exactly where its forward value is positive.  dbeta of a dy that is
+    one at a single channel counts them."""
+    from hific_amd import ops
+    x = _rand(shape, 58, scale=1.5)
+    gamma, beta = _rand((shape[1],), 59), 0.5 * _rand((shape[1],), 60)
+    gamma[3], gamma[5], beta[5], gamma[7] = 0.0, 0.0, -0.25, 1e-30
+    xd, gd, bd = x.to(dev).requires_grad_(), gamma.to(dev).requires_grad_(), beta.to(dev).requires_grad_()
+    y, a = ops.channel_norm8(xd, gd, bd, relu=True, fmt=fmt)
+    db, = torch.autograd.grad(y, bd, torch.ones_like(y), retain_graph=True)
+    open_ = (y.detach() > 0).double().sum([0] + list(range(2, len(shape))))
+    assert torch.equal(db.double(), open_)
+    assert 0.2 < float(open_.sum() / x.numel()) < 0.8
+    assert torch.equal(ops.restore8(a, torch.float32) > 0, y > 0)
+
+
 def test_channel_norm8_agrees_with_channel_norm(hific, dev):
     """y as channel_norm gives it (the same formula; another order of the sums), gradients within what 8 bits cost: xh is off by
     u = half a step <= 2^-7 * max|xh|, rms u / sqrt(3) - times the two places where xh enters dx."""
@@ -578,6 +596,63 @@ def test_captured_and_replayed(hific, dev):
             for k, (a, b) in enumerate(zip(out, step(x))):
                 assert torch.equal(a, b), (rep, k)
         torch.cuda.synchronize()
+
+
+def test_two_graphs_replayed_at_once(hific, dev):
+    """Two graphs captured on one stream and replayed on two streams at the same time share nothing that is written."""
+    from hific_amd import ops
+    shape = (4, 120, 32, 32)
+    gamma, beta = _chan(shape, 191).to(dev), _chan(shape, 192, 0.0).to(dev)
+    ins = [_rand(shape, 193 + i, torch.bfloat16).to(dev) for i in range(2)]
+    rstd = torch.rand(4, 32, 32, device=dev) + 0.5
+
+    def step(x):
+        with torch.no_grad():
+            y, a = ops.channel_norm8(x, gamma, beta, relu=True)
+            b8, h = ops.rms_norm8(x, gamma, resid=y)
+        dx, dg, db = ops.channel_norm_grad8(ops.Act8(a.q, a.e), x, gamma, beta, rstd, relu=True)
+        c = ops.checkpoint8(dx)
+        return (y, h, dx, dg, db, ops.restore8(b8), ops.conv2d_weight_grad8(c, y, (3, 3), pads=(1, 1, 1, 1)),
+                ops.conv2d_weight_grad8(c, y[:, :, :31, :31], (2, 2)))
+    st = torch.cuda.Stream()
+    want, graphs, outs = [], [], []
+    for x in ins:
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            want.append([t.clone() for t in step(x)])
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st, capture_error_mode="relaxed"):
+            outs.append(step(x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for rep in range(6):
+        for t in (t for o in outs for t in o):
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            for k, (p, q) in enumerate(zip(o, w)):
+                assert torch.equal(p, q), (rep, k)
+
+
+def test_many_small_planes(hific, dev):
+    """More images than a workgroup's share of tiles: workgroups cross image borders; the channel sums are those of each image alone."""
+    from hific_amd import ops
+    shape = (3000, 12, 3, 4)
+    x, w, dy = _rand(shape, 201, torch.bfloat16).to(dev), _chan(shape, 202).to(dev), _rand(shape, 203, torch.bfloat16).to(dev)
+    xd, wd = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = ops.rms_norm(xd, wd, fmt="int8")
+    q, e, rstd, _ = y.grad_fn.saved_tensors
+    dx, dw = torch.autograd.grad(y, (xd, wd), dy)
+    wdx, wdw = O.rms_norm_grad(O.values(q.cpu(), e.cpu()), rstd.cpu().double().unsqueeze(1), w.cpu(), dy.cpu())
+    _close(dx, wdx, _half(torch.bfloat16), 64 * F32, "dx")
+    _close(dw, wdw, 0.0, 8 * F32 * (dy.cpu().double() * O.values(q.cpu(), e.cpu())).abs().sum((0, 2, 3)), "dweight")
+    y1 = ops.rms_norm(x[1234:1235], w)
+    assert torch.equal(y1, y[1234:1235])
 
 
 def test_a_tensor_beyond_32_bit_offsets(hific, dev):
