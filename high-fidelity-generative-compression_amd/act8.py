@@ -158,7 +158,7 @@ def checkpoint8(x, fmt="int8"):
     code, dt = _fmt(fmt)
     N, C, HW = _nchw(x)
     _one_device(x)
-    x = c16(x.detach())
+    x = c16(x)
     cd = lib.dtype_code(x)
     q, e = _new8(x, dt)
     if N and HW:
@@ -389,7 +389,7 @@ def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
     _param(rstd, a.e.numel(), "rstd")
     lib.dtype_code(dy)
     dg, db = torch.empty_like(gamma), torch.empty_like(beta)
-    return _cn8_bwd(a.q, a.e, rstd, c16(dy.detach()), gamma, beta, bool(relu), dg, db, 0), dg, db
+    return _cn8_bwd(a.q, a.e, rstd, c16(dy), gamma, beta, bool(relu), dg, db, 0), dg, db
 
 
 # ---- training with 8-bit checkpoints ---------------------------------------------------------------------------------------------
@@ -685,7 +685,7 @@ def _wgrad_args(a, dy, kernel, name):
         raise lib.HificError(f"{name}: kernel {(R, S)} is not supported (1 to 64 taps)")
     _one_device(a.q, dy)
     lib.dtype_code(dy)
-    return R, S, c16(dy.detach())
+    return R, S, c16(dy)
 
 
 def conv2d_weight_grad8(a, dy, kernel, stride=1, pads=(0, 0, 0, 0), pad_mode=lib.PAD_ZERO):

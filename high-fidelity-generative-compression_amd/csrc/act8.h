@@ -273,7 +273,8 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
 // Tile of the plane kernels: 256 threads, LPX groups of eight positions, 256 / LPX channel groups, at most `most` channels per
 // thread, images of less than 4 GiB.  The widest LPX that fits the channels (what a tile costs besides its values - reductions,
 // scales, barriers - is shared by most values then: norm forward 16x60x256x256 75 us, with LPX <= 8 120), then narrower while
-// there are CUs without a workgroup (16x960x16x16: 256 wide tiles 12 us, 512 narrow ones 13.4).  lpx = 0: more channels than the
+// there are CUs without a workgroup (16x960x16x16: 256 wide tiles 12 us, 512 narrow ones 13.4) or more than an eighth of the lanes
+// lies past the planes' ends.  lpx = 0: more channels than the
 // registers hold, or images beyond 32-bit byte offsets.
 struct TileCfg { int lpx, cpt; unsigned tiles; long long blocks; };
 static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
@@ -285,7 +286,8 @@ static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
         t.lpx = lpx; t.cpt = cpt;
         t.tiles = (unsigned)cdiv(cdiv(HW, 8), lpx);
         t.blocks = (long long)t.tiles * N;
-        if (t.blocks >= 256 || cpt <= 1) break;
+        const long long octs = cdiv(HW, 8);
+        if ((t.blocks >= 256 || cpt <= 1) && (lpx == 1 || (long long)t.tiles * lpx * 8 <= octs * 9)) break;
     }
     return t;
 }
@@ -299,50 +301,53 @@ static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
 #define TILE_CPT(LPX, t, MOST, F)                                                                                         \
     if ((t).cpt <= 1) { F(LPX, 1); } else if ((t).cpt <= 2) { F(LPX, 2); } else if ((t).cpt <= 4) { F(LPX, 4); } else { F(LPX, ((MOST) < 8 ? 4 : 8)); }
 
-// Rows: L lanes and K groups of eight channels per lane hold a row.  Sums and maxima over the row's L lanes, through LDS where a
-// row has the whole workgroup.
-template <int L>
-__device__ __forceinline__ float row_sum(float v) {
+// Rows: L lanes and K groups of eight channels per lane hold a row, in workgroups of row_block(L) threads.  Sums and maxima over the
+// row's L lanes, through LDS where a row has the whole workgroup.
+constexpr int row_block(int L) { return L > 256 ? L : 256; }
+template <int L, typename V, typename Op>
+__device__ __forceinline__ V row_reduce(V v, Op op) {
 #pragma unroll
-    for (int o = (L < 64 ? L : 64) >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    if (L == 256) {
-        __shared__ float red[4];
+    for (int o = (L < 64 ? L : 64) >> 1; o > 0; o >>= 1) v = op(v, __builtin_bit_cast(V, __shfl_xor(__builtin_bit_cast(int, v), o, 64)));
+    if constexpr (L >= 256) {
+        __shared__ V red[L / 64];
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = (red[0] + red[1]) + (red[2] + red[3]);
-    }
-    return v;
-}
-template <int L>
-__device__ __forceinline__ unsigned row_max(unsigned v) {
+        V part[L / 64];
 #pragma unroll
-    for (int o = (L < 64 ? L : 64) >> 1; o > 0; o >>= 1) v = umax(v, (unsigned)__shfl_xor((int)v, o, 64));
-    if (L == 256) {
-        __shared__ unsigned red[4];
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = umax(umax(red[0], red[1]), umax(red[2], red[3]));
+        for (int i = 0; i < L / 64; ++i) part[i] = red[i];
+#pragma unroll
+        for (int s = L / 128; s > 0; s >>= 1)
+#pragma unroll
+            for (int i = 0; i < s; ++i) part[i] = op(part[i], part[i + s]);
+        v = part[0];
     }
     return v;
 }
-// 16 lanes for up to 128 channels, a wave for more, the whole workgroup for wide rows and where fewer than 1024 rows would leave
-// the other CUs idle.  l = 0: more channels than the registers hold.
+template <int L> __device__ __forceinline__ float row_sum(float v) { return row_reduce<L>(v, [](float a, float b) { return a + b; }); }
+template <int L> __device__ __forceinline__ unsigned row_max(unsigned v) { return row_reduce<L>(v, [](unsigned a, unsigned b) { return umax(a, b); }); }
+// As few lanes of a wave as hold the row in one group each (65536x129, both passes: 32 lanes 36 us, 64 lanes 52), the wave with up to 4 groups for
+// wider ones, a workgroup of 256 above 2048 channels and where fewer than 1024 rows would leave the other CUs idle, one of 1024
+// threads above 8192 (2048x16384, both passes: 126 us, the any-shape kernels 331).  l = 0: more channels than the registers hold.
 struct RowCfg { int l, k; };
 static inline RowCfg row_pick(long long N, int C) {
     RowCfg r;
-    r.l = C <= 128 ? 16 : ((C > 2048 || (N < 1024 && C > 512)) ? 256 : 64);
+    if (C > 2048 || (N < 1024 && C > 512)) r.l = C > 8192 ? 1024 : 256;
+    else r.l = C <= 64 ? 8 : (C <= 128 ? 16 : (C <= 256 ? 32 : 64));
     r.k = cdiv(C, 8 * r.l);
-    if (r.k > 4) r.l = 0;
+    if (r.k > (r.l == 1024 ? 2 : 4)) r.l = 0;
     return r;
 }
 #define ROW_DISPATCH(r, F)                                                                              \
     do {                                                                                                \
-        if ((r).l == 16) F(16, 1);                                                                      \
-        else if ((r).l == 64) { if ((r).k <= 1) F(64, 1); else if ((r).k <= 2) F(64, 2); else F(64, 4); } \
-        else if ((r).k <= 1) F(256, 1); else if ((r).k <= 2) F(256, 2); else F(256, 4);                 \
+        if ((r).l == 8) { F(8, 1); } else if ((r).l == 16) { F(16, 1); } else if ((r).l == 32) { F(32, 1); } \
+        else if ((r).l == 64) { if ((r).k <= 1) { F(64, 1); } else if ((r).k <= 2) { F(64, 2); } else { F(64, 4); } } \
+        else if ((r).l == 256) { if ((r).k <= 1) { F(256, 1); } else if ((r).k <= 2) { F(256, 2); } else { F(256, 4); } } \
+        else { F(1024, 2); }                                                                            \
     } while (0);
+
+// lanes on positions of the any-shape kernels (the rest of 256 on channels): 64, 16 where the planes are small or few, 1 for rows
+static inline int any_px(long long N, int HW) { return HW == 1 ? 1 : (HW < 48 || cdiv(HW, 64) * N < 512 ? 16 : 64); }
 
 static inline bool act8_dtype_ok(int dtype) { return dtype == HIFIC_F32 || dtype == HIFIC_BF16; }
 static inline bool act8_fmt_ok(int fmt) { return fmt == HIFIC_Q_INT8 || fmt == HIFIC_Q_E4M3; }

@@ -113,9 +113,9 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const u8_t* __restric
 
 // Rows (HW = 1) of eight channels and more: eight channels per lane, L lanes and K groups per lane for a row.
 template <typename T, int FMT, int L, int K>
-__global__ __launch_bounds__(256) void act8_pack_rows_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe, int N, int C) {
+__global__ __launch_bounds__(row_block(L)) void act8_pack_rows_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe, int N, int C) {
     const int l = threadIdx.x % L;
-    const long long row0 = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const long long row0 = (long long)blockIdx.x * (row_block(L) / L) + threadIdx.x / L;
     const bool ok = row0 < N;
     const size_t base = (size_t)(ok ? row0 : N - 1) * C;
     V8<T> xr[K];
@@ -179,12 +179,12 @@ int pack_launch(const T* x, u8_t* q, u8_t* qe, int N, int C, int HW, hipStream_t
     }
     RowCfg r;
     if (HW == 1 && C >= 8 && (r = row_pick(N, C)).l) {
-#define ROWS(L, K) hipLaunchKernelGGL((act8_pack_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, 256 / L)), dim3(256), 0, st, x, q, qe, N, C)
+#define ROWS(L, K) hipLaunchKernelGGL((act8_pack_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, row_block(L) / L)), dim3(row_block(L)), 0, st, x, q, qe, N, C)
         ROW_DISPATCH(r, ROWS)
 #undef ROWS
         return hific_launch_status();
     }
-    const int px = HW == 1 ? 1 : (HW < 48 ? 16 : 64);
+    const int px = any_px(N, HW);
     const long long tiles = cdivl(HW, px), blocks = tiles * N;
     if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)blocks);

@@ -39,6 +39,5 @@ __device__ __forceinline__ unsigned tok_max(unsigned v, float (*red)[PX]) {
     return umax(umax(__float_as_uint(red[0][p]), __float_as_uint(red[1][p])), umax(__float_as_uint(red[2][p]), __float_as_uint(red[3][p])));
 }
 
-inline int norm8_px(int HW) { return HW == 1 ? 1 : (HW < 48 ? 16 : 64); }       // lanes on positions of the any-shape kernels
 // channels per thread that the plane kernels keep in registers
 template <typename T> constexpr int tile_most() { return sizeof(T) == 2 ? 8 : 4; }

@@ -201,11 +201,11 @@ __global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p,
     }
 }
 
-// Rows: a workgroup takes every gridDim.x-th group of 256 / L rows and keeps the sums of its channels in registers.
+// Rows: a workgroup takes every gridDim.x-th group of R rows and keeps the sums of its channels in registers.
 template <typename T, int SRC, int L, int K>
-__global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int N) {
-    constexpr int R = 256 / L;
-    __shared__ float red[R][L][8];
+__global__ __launch_bounds__(row_block(L)) void rms_bwd_rows_kernel(const NormBwd p, int N) {
+    constexpr int R = row_block(L) / L;
+    __shared__ float red[R > 1 ? R : 1][R > 1 ? L : 1][8];
     const int l = threadIdx.x % L, rg = threadIdx.x / L;
     const unsigned C = p.C;
     V8<float> w[K];
@@ -251,6 +251,9 @@ __global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int 
                 s2 += d * w[k].get(j);
             }
         }
+        if constexpr (K > 1)             // (unpacked again below, as in norm8_bwd_tile_kernel)
+#pragma unroll
+            for (int k = 0; k < K; ++k) { dy[k].forget(); if constexpr (SRC == SRC_T) hr[k].forget(); else forget(q[k]); }
         s2 = row_sum<L>(s2) * p.rv;
         if (!ok) continue;               // (only the last round has rows that are not there, and none of its lanes waits again)
 #pragma unroll
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(256) void rms_bwd_rows_kernel(const NormBwd p, int 
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const unsigned cn = (unsigned)(l + L * k) * 8, c = umin(cn, C - 8);
-        if (R > 1) {
+        if constexpr (R > 1) {
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < 8; ++j) red[rg][l][j] = pg[k][j];
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(1024) void norm8_colsum_kernel(const float* __restr
 
 namespace {
 int norm8_nsplit(int N, int C, int HW) {                             // ~1024 workgroups, at least 64 tokens each
-    const int px = norm8_px(HW), cb = cdiv(C, 256 / px);
+    const int px = any_px(N, HW), cb = cdiv(C, 256 / px);
     const long long tokens = (long long)N * HW, most = cdivl(tokens, 64);
     long long s = cdiv(1024, cb);
     if (s > most) s = most;
@@ -345,7 +348,10 @@ size_t norm8_rows(int mode, int N, int C, int HW) {
     }
     if (mode == M_RMS && HW == 1 && C >= 8) {
         const RowCfg r = row_pick(N, C);
-        if (r.l) { const int g = cdiv(N, 256 / r.l); return (size_t)(g < 1024 ? g : 1024); }
+        if (r.l) {                       // at least four groups of rows per workgroup once every CU has one: each writes a row of C sums
+            const int g = cdiv(N, row_block(r.l) / r.l);
+            return (size_t)(g <= 256 ? g : (g < 1024 ? 256 : (g < 4096 ? cdiv(g, 4) : 1024)));
+        }
     }
     return (size_t)norm8_nsplit(N, C, HW);
 }
@@ -371,12 +377,12 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
 #undef BWD
     } else if (r.l) {
         if constexpr (MODE == M_RMS) {
-#define ROWS(L, K) hipLaunchKernelGGL((rms_bwd_rows_kernel<T, SRC, L, K>), dim3((unsigned)rows), dim3(256), 0, st, p, N)
+#define ROWS(L, K) hipLaunchKernelGGL((rms_bwd_rows_kernel<T, SRC, L, K>), dim3((unsigned)rows), dim3(row_block(L)), 0, st, p, N)
             ROW_DISPATCH(r, ROWS)
 #undef ROWS
         }
     } else {
-        const int px = norm8_px(p.HW);
+        const int px = any_px(N, p.HW);
         const long long blocks = cdivl(p.HW, px) * N;
         if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
         p.tiles = (unsigned)cdivl(p.HW, px);

@@ -247,10 +247,10 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
 
 // Rows of eight channels and more (root-mean-square norm): eight channels per lane, L lanes and K groups per lane for a row.
 template <typename T, int FMT, int L, int K>
-__global__ __launch_bounds__(256) void rms_fwd_rows_kernel(const NormFwd p, int N) {
+__global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFwd p, int N) {
     constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;
     const int l = threadIdx.x % L;
-    const long long row0 = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const long long row0 = (long long)blockIdx.x * (row_block(L) / L) + threadIdx.x / L;
     const bool ok = row0 < N;
     const size_t base = (size_t)(ok ? row0 : N - 1) * p.C;
     const unsigned C = p.C;
@@ -334,13 +334,13 @@ int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
     if constexpr (MODE == M_RMS) {
         RowCfg r;
         if (p.HW == 1 && p.C >= 8 && (r = row_pick(N, p.C)).l) {
-#define ROWS(L, K) hipLaunchKernelGGL((rms_fwd_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, 256 / L)), dim3(256), 0, st, p, N)
+#define ROWS(L, K) hipLaunchKernelGGL((rms_fwd_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, row_block(L) / L)), dim3(row_block(L)), 0, st, p, N)
             ROW_DISPATCH(r, ROWS)
 #undef ROWS
             return hific_launch_status();
         }
     }
-    const int px = norm8_px(p.HW);
+    const int px = any_px(N, p.HW);
     const long long blocks = cdivl(p.HW, px) * N;
     if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
     p.tiles = (unsigned)cdivl(p.HW, px);
