@@ -1,4 +1,4 @@
-"""Activations in 8 bits, the norms that write and read them, and the root-mean-square norm (csrc/act8.hip, csrc/norm8.hip).
+"""Activations in 8 bits, the norms that write and read them, and the root-mean-square norm (csrc/act8.hip, csrc/norm8_fwd.hip, csrc/norm8_bwd.hip).
 
 A token is one position of an activation [N, C, ...] (a pixel of [N, C, H, W], a row of [N, C]).  Its C values are held as int8 or
 e4m3 numbers with ONE power-of-two exponent per token, so a restored value is exact in bfloat16.  `Act8` is such an activation;
@@ -20,6 +20,7 @@ FORMATS = {"int8": (0, torch.int8), "e4m3": (1, torch.float8_e4m3fn)}
 _CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _INF = float("inf")
 _INT = 2 ** 31 - 1
+_MAX_C = 2 ** 20                          # channels that a token's sums and exponent are formed over; strides and pads
 
 
 def _fmt(fmt):
@@ -36,8 +37,8 @@ def _nchw(x, name="x"):
     n, c, hw = x.size(0), x.size(1), 1
     for i in range(2, d):
         hw *= x.size(i)
-    if n > _INT or c > _INT or hw > _INT:
-        raise lib.HificError(f"{name}: a dimension of {tuple(x.shape)} is beyond 32 bits")
+    if n > _INT or c > _MAX_C or hw > _INT:
+        raise lib.HificError(f"{name}: {tuple(x.shape)} has a dimension beyond 32 bits or more than {_MAX_C} channels")
     return n, c, hw
 
 
@@ -518,6 +519,8 @@ class ConvNorm8Fn(Function):
         require_gpu(x, weight, bias, gamma, beta, resid)
         with _on(x):
             z = _conv_fwd(x, weight, bias, geom, False)
+            _param(gamma, z.size(1), "gamma")
+            _param(beta, z.size(1), "beta")
             if resid is not None:
                 _like(resid, z, "resid")
             y, rstd, nq, ne, q2, e2 = _cn8_fwd(z, gamma, beta, resid, eps, relu, _nchw(z), lib.dtype_code(z), code, dt)
@@ -575,6 +578,7 @@ def _split8(x8, x):
         return None, None, None, None, False
     if not isinstance(x8, Act8) or x8.shape != x.shape:
         raise lib.HificError(f"x8 must be the Act8 of x {tuple(x.shape)}")
+    _one_device(x, x8.q)
     return x8.q, x8.e, x8.gamma, x8.beta, x8.relu
 
 
@@ -696,7 +700,7 @@ def conv2d_weight_grad8(a, dy, kernel, stride=1, pads=(0, 0, 0, 0), pad_mode=lib
     N, C, H, W = a.shape
     pt, pl, pb, pr = (int(v) for v in pads)
     stride = int(stride)
-    if stride < 1 or min(pt, pl, pb, pr) < 0 or pad_mode not in (lib.PAD_ZERO, lib.PAD_REFLECT):
+    if not 1 <= stride <= _MAX_C or min(pt, pl, pb, pr) < 0 or max(pt, pl, pb, pr) > _MAX_C or pad_mode not in (lib.PAD_ZERO, lib.PAD_REFLECT):
         raise lib.HificError("conv2d_weight_grad8: bad stride, pads or pad_mode")
     if pad_mode == lib.PAD_REFLECT and (max(pt, pb) >= H or max(pl, pr) >= W):
         raise lib.HificError("conv2d_weight_grad8: reflection pads must be smaller than the plane")
@@ -716,7 +720,7 @@ def conv_transpose2d_weight_grad8(a, dy, kernel, stride, pad, outpad):
     R, S, dy = _wgrad_args(a, dy, kernel, "conv_transpose2d_weight_grad8")
     N, C, H, W = a.shape
     stride, pad, outpad = int(stride), int(pad), int(outpad)
-    if stride < 1 or pad < 0 or outpad < 0:
+    if not 1 <= stride <= _MAX_C or not 0 <= pad <= _MAX_C or not 0 <= outpad <= _MAX_C:
         raise lib.HificError("conv_transpose2d_weight_grad8: bad stride or padding")
     size = ((H - 1) * stride - 2 * pad + R + outpad, (W - 1) * stride - 2 * pad + S + outpad)
     if min(size) < 1 or tuple(dy.shape[2:]) != size:

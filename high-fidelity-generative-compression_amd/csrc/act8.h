@@ -1,5 +1,5 @@
-// Activations held in 8 bits: number formats, token addressing and reductions shared by act8.hip (checkpoints) and norm8.hip
-// (norms that write or read them).
+// Activations held in 8 bits: number formats, token addressing and reductions shared by act8.hip (checkpoints),
+// norm8_fwd.hip and norm8_bwd.hip (norms that write or read them).
 //
 // A token is one position of an activation [N, C, HW]; its C values share ONE exponent.  q is int8 or e4m3 (finite-only,
 // largest value 448), shape of the tensor; qe [N, HW] holds exponent + 127 in a byte:
@@ -276,7 +276,7 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
 // there are CUs without a workgroup (16x960x16x16: 256 wide tiles 12 us, 512 narrow ones 13.4) or more than an eighth of the lanes
 // lies past the planes' ends.  lpx = 0: more channels than the
 // registers hold, or images beyond 32-bit byte offsets.
-struct TileCfg { int lpx, cpt; unsigned tiles; long long blocks; };
+struct TileCfg { int lpx, cpt; unsigned tiles; long long blocks; };      // (tiles per image, less than 2^20; of the batch)
 static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
     TileCfg t{0, 0, 0, 0};
     if ((long long)(C + 256) * HW > (1ll << 30) - 64) return t;      // (C + 256: a lane's offset is formed before it is dropped)
@@ -346,8 +346,24 @@ static inline RowCfg row_pick(long long N, int C) {
         else { F(1024, 2); }                                                                            \
     } while (0);
 
-// lanes on positions of the any-shape kernels (the rest of 256 on channels): 64, 16 where the planes are small or few, 1 for rows
-static inline int any_px(long long N, int HW) { return HW == 1 ? 1 : (HW < 48 || cdiv(HW, 64) * N < 512 ? 16 : 64); }
+// Lanes on tokens of the any-shape kernels, counted over the batch (the rest of 256 on channels): 64, 16 where they are few, 1 for
+// rows of eight channels and more, whose neighbours in memory are channels.  At most 2^20 workgroups, each with its share of the tokens.
+static inline int any_px(long long N, int C, int HW) { return HW == 1 && C >= 8 ? 1 : (N * HW < 64 * 512 ? 16 : 64); }
+static inline unsigned any_grid(long long blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20); }
 
+// A launch holds less than 2^32 threads: F(first image, images) over parts of the batch of at most 2^21 workgroups (or one image).
+template <typename F>
+static inline int batch_parts(long long N, long long per_image, F f) {
+    const long long step = (1ll << 21) / per_image > 1 ? (1ll << 21) / per_image : 1;
+    for (long long n = 0; n < N; n += step) {
+        const int rc = f(n, N - n < step ? N - n : step);
+        if (rc != HIFIC_OK) return rc;
+    }
+    return HIFIC_OK;
+}
+// a null pointer stays one
+template <typename T> static inline T* ahead(T* p, long long n) { return p ? p + n : p; }
+
+constexpr int ACT8_MAX_C = 1 << 20;      // channels of a token in what forms its sums or exponent
 static inline bool act8_dtype_ok(int dtype) { return dtype == HIFIC_F32 || dtype == HIFIC_BF16; }
 static inline bool act8_fmt_ok(int fmt) { return fmt == HIFIC_Q_INT8 || fmt == HIFIC_Q_E4M3; }

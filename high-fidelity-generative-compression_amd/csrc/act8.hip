@@ -2,26 +2,29 @@
 // writes 1 byte per element, restore the reverse.
 #include "act8.h"
 
-// Any shape: PX lanes on consecutive positions x 256 / PX channel groups, the tensor read twice (the second time from L2).
+// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor read twice (the second time from L2).
 template <typename T, int FMT, int PX>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
-                                                        int C, int HW, unsigned tiles) {
+                                                        int C, int HW, long long tokens) {
     constexpr int G = 256 / PX;
     __shared__ unsigned red[G][PX];
     const int px = threadIdx.x % PX, g = threadIdx.x / PX;
-    const unsigned n = blockIdx.x / tiles, hw = (blockIdx.x - n * tiles) * PX + px;
-    const bool ok = hw < (unsigned)HW;
-    const size_t base = (size_t)n * C * HW + (ok ? hw : 0);
-    unsigned am = 0;
-    for (int c = g; c < C; c += G) am = umax(am, abs_bits(DT<T>::ld(x + base + (size_t)c * HW)));
-    red[g][px] = am;
-    __syncthreads();
-    for (int k = 0; k < G; ++k) am = umax(am, red[k][px]);
-    const unsigned code = q8_code<FMT>(am);
-    const float inv = q8_inv_scale(code);
-    if (!ok) return;
-    if (g == 0) qe[(size_t)n * HW + hw] = (u8_t)code;
-    for (int c = g; c < C; c += G) q[base + (size_t)c * HW] = (u8_t)q8_round<FMT>(DT<T>::ld(x + base + (size_t)c * HW) * inv);
+    for (long long t0 = (long long)blockIdx.x * PX; t0 < tokens; t0 += (long long)gridDim.x * PX) {
+        const bool ok = t0 + px < tokens;
+        const long long tok = ok ? t0 + px : tokens - 1, n = tok / HW;
+        const size_t base = (size_t)n * C * HW + (size_t)(tok - n * HW);
+        unsigned am = 0;
+        for (int c = g; c < C; c += G) am = umax(am, abs_bits(DT<T>::ld(x + base + (size_t)c * HW)));
+        __syncthreads();
+        red[g][px] = am;
+        __syncthreads();
+        for (int k = 0; k < G; ++k) am = umax(am, red[k][px]);
+        const unsigned code = q8_code<FMT>(am);
+        const float inv = q8_inv_scale(code);
+        if (!ok) continue;               // (the last round only)
+        if (g == 0) qe[tok] = (u8_t)code;
+        for (int c = g; c < C; c += G) q[base + (size_t)c * HW] = (u8_t)q8_round<FMT>(DT<T>::ld(x + base + (size_t)c * HW) * inv);
+    }
 }
 
 // Planes of eight positions and more: the tile stays in registers between the maximum and the rounding, one pass over HBM.
@@ -169,28 +172,32 @@ int pack_launch(const T* x, u8_t* q, u8_t* qe, int N, int C, int HW, hipStream_t
     if (HW >= 8) {
         const TileCfg t = tile_pick(N, C, HW, 8);
         if (t.lpx) {
-            if (t.blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-            const dim3 grid((unsigned)t.blocks);
-#define TILE(LPX, CPT) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT>), grid, dim3(256), 0, st, x, q, qe, C, HW, t.tiles, (unsigned)t.blocks)
-            TILE_DISPATCH(t, 8, TILE);
+            return batch_parts(N, t.tiles, [&](long long n0, long long n) {
+                const long long at = n0 * C * HW;
+                const unsigned blocks = (unsigned)(t.tiles * n);
+#define TILE(LPX, CPT) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT>), dim3(blocks), dim3(256), 0, st, x + at, q + at, qe + n0 * HW, C, HW, t.tiles, blocks)
+                TILE_DISPATCH(t, 8, TILE);
 #undef TILE
-            return hific_launch_status();
+                return hific_launch_status();
+            });
         }
     }
     RowCfg r;
     if (HW == 1 && C >= 8 && (r = row_pick(N, C)).l) {
-#define ROWS(L, K) hipLaunchKernelGGL((act8_pack_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, row_block(L) / L)), dim3(row_block(L)), 0, st, x, q, qe, N, C)
-        ROW_DISPATCH(r, ROWS)
+        return batch_parts(N, 1, [&](long long n0, long long n) {
+            const long long at = n0 * C;
+#define ROWS(L, K) hipLaunchKernelGGL((act8_pack_rows_kernel<T, FMT, L, K>), dim3(cdiv((int)n, row_block(L) / L)), dim3(row_block(L)), 0, st, x + at, q + at, qe + n0, (int)n, C)
+            ROW_DISPATCH(r, ROWS)
 #undef ROWS
-        return hific_launch_status();
+            return hific_launch_status();
+        });
     }
-    const int px = any_px(N, HW);
-    const long long tiles = cdivl(HW, px), blocks = tiles * N;
-    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)blocks);
-    if (px == 1) hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 1>), grid, dim3(256), 0, st, x, q, qe, C, HW, (unsigned)tiles);
-    else if (px == 16) hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 16>), grid, dim3(256), 0, st, x, q, qe, C, HW, (unsigned)tiles);
-    else hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 64>), grid, dim3(256), 0, st, x, q, qe, C, HW, (unsigned)tiles);
+    const int px = any_px(N, C, HW);
+    const long long tokens = (long long)N * HW;
+    const dim3 grid(any_grid(cdivl(tokens, px)));
+    if (px == 1) hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 1>), grid, dim3(256), 0, st, x, q, qe, C, HW, tokens);
+    else if (px == 16) hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 16>), grid, dim3(256), 0, st, x, q, qe, C, HW, tokens);
+    else hipLaunchKernelGGL((act8_pack_kernel<T, FMT, 64>), grid, dim3(256), 0, st, x, q, qe, C, HW, tokens);
     return hific_launch_status();
 }
 
@@ -198,18 +205,24 @@ template <typename T, int FMT>
 int restore_launch(const u8_t* q, const u8_t* qe, const float* gamma, const float* beta, int relu, T* out, int N, int C, int HW, hipStream_t st) {
     if (HW == 1 && C >= 8) {
         const unsigned octs = (unsigned)cdiv(C, 8);
-        const long long n = (long long)octs * N, blocks = cdivl(n, 256);
-        if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-        hipLaunchKernelGGL((act8_restore_rows_kernel<T, FMT>), dim3((unsigned)blocks), dim3(256), 0, st, q, qe, gamma, beta, out, C, octs, n, relu);
-        return hific_launch_status();
+        return batch_parts(N, cdivl(octs, 256), [&](long long n0, long long n) {
+            const long long at = n0 * C;
+            hipLaunchKernelGGL((act8_restore_rows_kernel<T, FMT>), dim3((unsigned)cdivl(octs * n, 256)), dim3(256), 0, st, q + at, qe + n0, gamma, beta,
+                               out + at, C, octs, octs * n, relu);
+            return hific_launch_status();
+        });
     }
     constexpr int CH = 4;
     const unsigned octs = HW >= 8 ? (unsigned)cdiv(HW, 8) : (unsigned)HW, cgs = (unsigned)cdiv(C, CH);
-    const long long n = (long long)octs * cgs * N, blocks = cdivl(n, 256);
-    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-    if (HW >= 8) hipLaunchKernelGGL((act8_restore_kernel<T, FMT, 8, CH>), dim3((unsigned)blocks), dim3(256), 0, st, q, qe, gamma, beta, out, C, HW, octs, cgs, n, relu);
-    else hipLaunchKernelGGL((act8_restore_kernel<T, FMT, 1, CH>), dim3((unsigned)blocks), dim3(256), 0, st, q, qe, gamma, beta, out, C, HW, octs, cgs, n, relu);
-    return hific_launch_status();
+    const long long each = (long long)octs * cgs;                     // threads of an image
+    if (cdivl(each, 256) >= 1ll << 24) return HIFIC_ERR_UNSUPPORTED;  // (an image of more than 10^11 values)
+    return batch_parts(N, cdivl(each, 256), [&](long long n0, long long n) {
+        const long long at = n0 * C * HW, threads = each * n;
+        const dim3 grid((unsigned)cdivl(threads, 256));
+        if (HW >= 8) hipLaunchKernelGGL((act8_restore_kernel<T, FMT, 8, CH>), grid, dim3(256), 0, st, q + at, qe + n0 * HW, gamma, beta, out + at, C, HW, octs, cgs, threads, relu);
+        else hipLaunchKernelGGL((act8_restore_kernel<T, FMT, 1, CH>), grid, dim3(256), 0, st, q + at, qe + n0 * HW, gamma, beta, out + at, C, HW, octs, cgs, threads, relu);
+        return hific_launch_status();
+    });
 }
 }  // namespace
 
@@ -217,6 +230,7 @@ extern "C" {
 
 int hific_act8_pack(const void* x, void* q, void* qe, int fmt, int N, int C, int HW, int dtype, hipStream_t st) {
     if (!x || !q || !qe || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
+    if (C > ACT8_MAX_C) return HIFIC_ERR_UNSUPPORTED;
 #define PACK(T) (fmt == HIFIC_Q_INT8 ? pack_launch<T, HIFIC_Q_INT8>((const T*)x, (u8_t*)q, (u8_t*)qe, N, C, HW, st) \
                                      : pack_launch<T, HIFIC_Q_E4M3>((const T*)x, (u8_t*)q, (u8_t*)qe, N, C, HW, st))
     return dtype == HIFIC_F32 ? PACK(float) : PACK(bf16_t);

@@ -6,7 +6,7 @@ struct NormBwd {
     const float* rstd; const void* dy; const void* dstream; const float* w; const float* b;
     void* dx; float* part;
     int C, HW; unsigned tiles; int relu, db;
-    long long tokens; int nsplit;
+    long long tokens; int nsplit;        // (tokens: tiles of the batch in norm8_bwd_tile_kernel)
     float rc, rv;                        // as in NormFwd
 };
 
@@ -21,32 +21,34 @@ __global__ __launch_bounds__(256) void norm8_bwd_kernel(const NormBwd p) {
     constexpr int G = 256 / PX;
     __shared__ float red[4][PX];
     const int px = threadIdx.x % PX, g = threadIdx.x / PX;
-    const unsigned n = blockIdx.x / p.tiles, hw = (blockIdx.x - n * p.tiles) * PX + px;
-    const bool ok = hw < (unsigned)p.HW;
-    const size_t base = (size_t)n * p.C * p.HW + (ok ? hw : 0), tok = (size_t)n * p.HW + (ok ? hw : 0);
-    const T* dy = (const T*)p.dy + base;
     const size_t cs = p.HW;
-    const float r = p.rstd[tok], scale = SRC == SRC_T ? 0.f : q8_scale(p.qe[tok]);
-    float s1 = 0.f, s2 = 0.f;
-    for (int c = g; c < p.C; c += G) {
-        const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
-        float d = DT<T>::ld(dy + c * cs);
-        if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
-        d *= p.w[c];
-        s1 += d; s2 += d * xh;
-    }
-    if (MODE == M_CHAN) s1 = tok_sum<PX>(s1, red) * p.rc;
-    s2 = tok_sum<PX>(s2, red) * p.rv;
-    if (!ok) return;
-    for (int c = g; c < p.C; c += G) {
-        const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
-        float d = DT<T>::ld(dy + c * cs);
-        if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
-        d = d * p.w[c] - xh * s2;
-        if (MODE == M_CHAN) d -= s1;
-        d *= r;
-        if (MODE == M_RMS && p.dstream) d += DT<T>::ld((const T*)p.dstream + base + c * cs);
-        DT<T>::st((T*)p.dx + base + c * cs, d);
+    for (long long t0 = (long long)blockIdx.x * PX; t0 < p.tokens; t0 += (long long)gridDim.x * PX) {
+        const bool ok = t0 + px < p.tokens;
+        const long long tok = ok ? t0 + px : p.tokens - 1, n = tok / p.HW;
+        const size_t base = (size_t)n * p.C * p.HW + (size_t)(tok - n * p.HW);
+        const T* dy = (const T*)p.dy + base;
+        const float r = p.rstd[tok], scale = SRC == SRC_T ? 0.f : q8_scale(p.qe[tok]);
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = g; c < p.C; c += G) {
+            const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
+            float d = DT<T>::ld(dy + c * cs);
+            if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
+            d *= p.w[c];
+            s1 += d; s2 += d * xh;
+        }
+        if (MODE == M_CHAN) s1 = tok_sum<PX>(s1, red) * p.rc;
+        s2 = tok_sum<PX>(s2, red) * p.rv;
+        if (!ok) continue;               // (the last round only)
+        for (int c = g; c < p.C; c += G) {
+            const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
+            float d = DT<T>::ld(dy + c * cs);
+            if (MODE == M_CHAN && p.relu && !relu_on(fmaf(p.w[c], xh, p.b[c]))) d = 0.f;
+            d = d * p.w[c] - xh * s2;
+            if (MODE == M_CHAN) d -= s1;
+            d *= r;
+            if (MODE == M_RMS && p.dstream) d += DT<T>::ld((const T*)p.dstream + base + c * cs);
+            DT<T>::st((T*)p.dx + base + c * cs, d);
+        }
     }
 }
 
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(1024) void norm8_colsum_kernel(const float* __restr
 
 namespace {
 int norm8_nsplit(int N, int C, int HW) {                             // ~1024 workgroups, at least 64 tokens each
-    const int px = any_px(N, HW), cb = cdiv(C, 256 / px);
+    const int px = any_px(N, C, HW), cb = cdiv(C, 256 / px);
     const long long tokens = (long long)N * HW, most = cdivl(tokens, 64);
     long long s = cdiv(1024, cb);
     if (s > most) s = most;
@@ -382,13 +384,10 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
 #undef ROWS
         }
     } else {
-        const int px = any_px(N, p.HW);
-        const long long blocks = cdivl(p.HW, px) * N;
-        if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-        p.tiles = (unsigned)cdivl(p.HW, px);
+        const int px = any_px(N, p.C, p.HW);
         p.tokens = (long long)N * p.HW;
         p.nsplit = (int)rows;
-        const dim3 grid((unsigned)blocks), pgrid(cdiv(p.C, 256 / px), p.nsplit);
+        const dim3 grid(any_grid(cdivl(p.tokens, px))), pgrid(cdiv(p.C, 256 / px), p.nsplit);
 #define BWD(PX)                                                                                                 \
         do {                                                                                                    \
             hipLaunchKernelGGL((norm8_bwd_kernel<T, MODE, SRC, PX>), grid, dim3(256), 0, st, p);               \
@@ -405,14 +404,13 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
 extern "C" {
 
 size_t hific_norm8_bwd_ws_bytes(int N, int C, int HW) {
-    if (N <= 0 || C <= 0 || HW <= 0) return 0;
-    size_t rows = 0;
+    if (N <= 0 || C <= 0 || HW <= 0 || C > ACT8_MAX_C) return 0;
+    size_t rows = 0;                     // of C sums: one kind of them for the root-mean-square norm, up to three for the channel norm
     for (int mode : {M_RMS, M_CHAN}) {
-        const size_t a = norm8_rows<float>(mode, N, C, HW), b = norm8_rows<bf16_t>(mode, N, C, HW);
-        rows = a > rows ? a : rows;
-        rows = b > rows ? b : rows;
+        const size_t a = norm8_rows<float>(mode, N, C, HW), b = norm8_rows<bf16_t>(mode, N, C, HW), m = (a > b ? a : b) * (mode == M_RMS ? 1 : 3);
+        rows = m > rows ? m : rows;
     }
-    return rows * 3 * C * sizeof(float);
+    return rows * C * sizeof(float);
 }
 
 int hific_rms_norm_bwd(const void* h, const void* q, const void* qe, int fmt, const float* rstd, const void* dy, const void* dstream,
@@ -420,6 +418,7 @@ int hific_rms_norm_bwd(const void* h, const void* q, const void* qe, int fmt, co
                        hipStream_t st) {
     if (!rstd || !dy || !w || !dx || !dw || !ws || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype)) return HIFIC_ERR_ARG;
     if ((h != nullptr) == (q != nullptr) || (q != nullptr) != (qe != nullptr) || (q && !act8_fmt_ok(fmt))) return HIFIC_ERR_ARG;
+    if (C > ACT8_MAX_C) return HIFIC_ERR_UNSUPPORTED;
     NormBwd p{h, (const u8_t*)q, (const u8_t*)qe, rstd, dy, dstream, w, nullptr, dx, (float*)ws, C, HW, 0, 0, 0, 0, 0, 0.f, 0.f};
 #define RMS(T) (h ? norm8_bwd_launch<T, M_RMS, SRC_T>(p, N, dw, nullptr, nullptr, accumulate, 0, ws_bytes, st)              \
                   : fmt == HIFIC_Q_INT8                                                                                     \
@@ -434,6 +433,7 @@ int hific_channelnorm8_bwd(const void* q, const void* qe, int fmt, const float* 
                            int accumulate_prev, int N, int C, int HW, int relu, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
     if (!q || !qe || !rstd || !dy || !gamma || !beta || !dx || !dgamma || !dbeta || !ws || N <= 0 || C < 2 || HW <= 0) return HIFIC_ERR_ARG;
     if (!act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
+    if (C > ACT8_MAX_C) return HIFIC_ERR_UNSUPPORTED;
     NormBwd p{nullptr, (const u8_t*)q, (const u8_t*)qe, rstd, dy, nullptr, gamma, beta, dx, (float*)ws, C, HW, 0, relu,
               dprev_bias ? 1 : 0, 0, 0, 0.f, 0.f};
 #define CN(T) (fmt == HIFIC_Q_INT8                                                                                                       \

@@ -9,76 +9,78 @@ struct NormFwd {
     float rc, rv;                        // 1 / C, and 1 / C or 1 / (C - 1): a product in the place of a division per position
 };
 
-// Any shape: PX lanes on consecutive positions x 256 / PX channel groups, the tensor re-read by every pass (from L2).
+// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2).
 template <typename T, int MODE, int FMT, int PX>
-__global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p) {
+__global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long long tokens) {
     constexpr int G = 256 / PX;
     constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;
     __shared__ float red[4][PX];
     const int px = threadIdx.x % PX, g = threadIdx.x / PX;
-    const unsigned n = blockIdx.x / p.tiles, hw = (blockIdx.x - n * p.tiles) * PX + px;
-    const bool ok = hw < (unsigned)p.HW;
-    const size_t base = (size_t)n * p.C * p.HW + (ok ? hw : 0), tok = (size_t)n * p.HW + hw;
-    const T* x = (const T*)p.x + base;
-    const T* rs = p.resid ? (const T*)p.resid + base : nullptr;
-    T* y = p.y ? (T*)p.y + base : nullptr;
-    T* h = p.h ? (T*)p.h + base : nullptr;
     const size_t cs = p.HW;
-    auto stream = [&](int c) {
-        float v = DT<T>::ld(x + c * cs);
-        if (MODE == M_RMS && rs) { T o; DT<T>::st(&o, v + DT<T>::ld(rs + c * cs)); v = DT<T>::ld(&o); }
-        return v;
-    };
-    float mu = 0.f;
-    if (MODE == M_CHAN) {
-        float s = 0.f;
-        for (int c = g; c < p.C; c += G) s += stream(c);
-        mu = tok_sum<PX>(s, red) * p.rc;
-    }
-    float ss = 0.f;
-    for (int c = g; c < p.C; c += G) {
-        const float v = stream(c), d = v - mu;
-        ss += d * d;
-        if (MODE == M_RMS && h && ok) DT<T>::st(h + c * cs, v);
-    }
-    ss = tok_sum<PX>(ss, red);
-    const float r = rsqrtf(ss * p.rv + p.eps);
-    if (p.rstd && ok && g == 0) p.rstd[tok] = r;
-    unsigned code = 0;
-    float inv = 0.f, scale = 0.f;
-    if (FMT != Q_NONE) {
-        unsigned am = 0;
+    for (long long t0 = (long long)blockIdx.x * PX; t0 < tokens; t0 += (long long)gridDim.x * PX) {
+        const bool ok = t0 + px < tokens;
+        const long long tok = ok ? t0 + px : tokens - 1, n = tok / p.HW;
+        const size_t base = (size_t)n * p.C * p.HW + (size_t)(tok - n * p.HW);
+        const T* x = (const T*)p.x + base;
+        const T* rs = p.resid ? (const T*)p.resid + base : nullptr;
+        T* y = p.y ? (T*)p.y + base : nullptr;
+        T* h = p.h ? (T*)p.h + base : nullptr;
+        auto stream = [&](int c) {
+            float v = DT<T>::ld(x + c * cs);
+            if (MODE == M_RMS && rs) { T o; DT<T>::st(&o, v + DT<T>::ld(rs + c * cs)); v = DT<T>::ld(&o); }
+            return v;
+        };
+        float mu = 0.f;
+        if (MODE == M_CHAN) {
+            float s = 0.f;
+            for (int c = g; c < p.C; c += G) s += stream(c);
+            mu = tok_sum<PX>(s, red) * p.rc;
+        }
+        float ss = 0.f;
+        for (int c = g; c < p.C; c += G) {
+            const float v = stream(c), d = v - mu;
+            ss += d * d;
+            if (MODE == M_RMS && h && ok) DT<T>::st(h + c * cs, v);
+        }
+        ss = tok_sum<PX>(ss, red);
+        const float r = rsqrtf(ss * p.rv + p.eps);
+        if (p.rstd && ok && g == 0) p.rstd[tok] = r;
+        unsigned code = 0;
+        float inv = 0.f, scale = 0.f;
+        if (FMT != Q_NONE) {
+            unsigned am = 0;
+            for (int c = g; c < p.C; c += G) {
+                const float xh = (stream(c) - mu) * r;
+                am = umax(am, abs_bits(MODE == M_RMS && p.q_of_y ? xh * p.w[c] : xh));
+            }
+            code = q8_code<F>(tok_max<PX>(am, red));
+            inv = q8_inv_scale(code); scale = q8_scale(code);
+            if (ok && g == 0) p.qe[tok] = (u8_t)code;
+        }
+        unsigned am2 = 0;
         for (int c = g; c < p.C; c += G) {
             const float xh = (stream(c) - mu) * r;
-            am = umax(am, abs_bits(MODE == M_RMS && p.q_of_y ? xh * p.w[c] : xh));
+            float o = MODE == M_RMS ? xh * p.w[c] : fmaf(p.w[c], xh, p.b[c]);
+            if (FMT != Q_NONE && ok)
+                p.q[base + c * cs] = (u8_t)(MODE == M_CHAN && p.relu ? q8_round_masked<F>(xh, inv, scale, p.w[c], p.b[c])
+                                                                     : q8_round<F>((MODE == M_RMS && p.q_of_y ? o : xh) * inv));
+            if (MODE == M_CHAN && p.relu) o = relu_nan(o);
+            if (MODE == M_CHAN && rs) {      // both terms rounded to the storage type first, as norm and add one after the other
+                T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
+            }
+            if (y && ok) DT<T>::st(y + c * cs, o);
+            am2 = umax(am2, abs_bits(o));
         }
-        code = q8_code<F>(tok_max<PX>(am, red));
-        inv = q8_inv_scale(code); scale = q8_scale(code);
-        if (ok && g == 0) p.qe[tok] = (u8_t)code;
-    }
-    unsigned am2 = 0;
-    for (int c = g; c < p.C; c += G) {
-        const float xh = (stream(c) - mu) * r;
-        float o = MODE == M_RMS ? xh * p.w[c] : fmaf(p.w[c], xh, p.b[c]);
-        if (FMT != Q_NONE && ok)
-            p.q[base + c * cs] = (u8_t)(MODE == M_CHAN && p.relu ? q8_round_masked<F>(xh, inv, scale, p.w[c], p.b[c])
-                                                                 : q8_round<F>((MODE == M_RMS && p.q_of_y ? o : xh) * inv));
-        if (MODE == M_CHAN && p.relu) o = relu_nan(o);
-        if (MODE == M_CHAN && rs) {      // both terms rounded to the storage type first, as norm and add one after the other
-            T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
-        }
-        if (y && ok) DT<T>::st(y + c * cs, o);
-        am2 = umax(am2, abs_bits(o));
-    }
-    if (MODE == M_CHAN && FMT != Q_NONE && p.q2) {
-        const unsigned code2 = q8_code<F>(tok_max<PX>(am2, red));
-        const float inv2 = q8_inv_scale(code2);
-        if (ok && g == 0) p.qe2[tok] = (u8_t)code2;
-        for (int c = g; c < p.C; c += G) {
-            float o = fmaf(p.w[c], (stream(c) - mu) * r, p.b[c]);
-            if (p.relu) o = relu_nan(o);
-            T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
-            if (ok) p.q2[base + c * cs] = (u8_t)q8_round<F>(o * inv2);
+        if (MODE == M_CHAN && FMT != Q_NONE && p.q2) {
+            const unsigned code2 = q8_code<F>(tok_max<PX>(am2, red));
+            const float inv2 = q8_inv_scale(code2);
+            if (ok && g == 0) p.qe2[tok] = (u8_t)code2;
+            for (int c = g; c < p.C; c += G) {
+                float o = fmaf(p.w[c], (stream(c) - mu) * r, p.b[c]);
+                if (p.relu) o = relu_nan(o);
+                T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
+                if (ok) p.q2[base + c * cs] = (u8_t)q8_round<F>(o * inv2);
+            }
         }
     }
 }
@@ -311,6 +313,14 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
 }
 
 namespace {
+template <typename T>
+NormFwd norm8_part(NormFwd p, long long n0) {                        // from image n0 on
+    const long long i = n0 * p.C * p.HW, t = n0 * p.HW;
+    p.x = (const T*)p.x + i; p.resid = ahead((const T*)p.resid, i); p.y = ahead((T*)p.y, i); p.h = ahead((T*)p.h, i);
+    p.rstd = ahead(p.rstd, t);
+    p.q = ahead(p.q, i); p.qe = ahead(p.qe, t); p.q2 = ahead(p.q2, i); p.qe2 = ahead(p.qe2, t);
+    return p;
+}
 template <typename T, int MODE, int FMT>
 int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
     p.rc = 1.f / (float)p.C;
@@ -318,36 +328,39 @@ int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
     if (p.HW >= 8) {
         const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>());
         if (t.lpx) {
-            if (t.blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
             p.tiles = t.tiles;
-            const dim3 grid((unsigned)t.blocks);
+            return batch_parts(N, t.tiles, [&](long long n0, long long n) {
+                const NormFwd part = norm8_part<T>(p, n0);
+                const dim3 grid((unsigned)(t.tiles * n));
 #define FWD(LPX, CPT)                                                                                                               \
-            do {                                                                                                                    \
-                if (p.resid) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, true, LPX, CPT>), grid, dim3(256), 0, st, p, grid.x); \
-                else hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, false, LPX, CPT>), grid, dim3(256), 0, st, p, grid.x);  \
-            } while (0)
-            TILE_DISPATCH(t, tile_most<T>(), FWD);
+                do {                                                                                                                \
+                    if (p.resid) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, true, LPX, CPT>), grid, dim3(256), 0, st, part, grid.x); \
+                    else hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, false, LPX, CPT>), grid, dim3(256), 0, st, part, grid.x); \
+                } while (0)
+                TILE_DISPATCH(t, tile_most<T>(), FWD);
 #undef FWD
-            return hific_launch_status();
+                return hific_launch_status();
+            });
         }
     }
     if constexpr (MODE == M_RMS) {
         RowCfg r;
         if (p.HW == 1 && p.C >= 8 && (r = row_pick(N, p.C)).l) {
-#define ROWS(L, K) hipLaunchKernelGGL((rms_fwd_rows_kernel<T, FMT, L, K>), dim3(cdiv(N, row_block(L) / L)), dim3(row_block(L)), 0, st, p, N)
-            ROW_DISPATCH(r, ROWS)
+            return batch_parts(N, 1, [&](long long n0, long long n) {
+                const NormFwd part = norm8_part<T>(p, n0);
+#define ROWS(L, K) hipLaunchKernelGGL((rms_fwd_rows_kernel<T, FMT, L, K>), dim3(cdiv((int)n, row_block(L) / L)), dim3(row_block(L)), 0, st, part, (int)n)
+                ROW_DISPATCH(r, ROWS)
 #undef ROWS
-            return hific_launch_status();
+                return hific_launch_status();
+            });
         }
     }
-    const int px = any_px(N, p.HW);
-    const long long blocks = cdivl(p.HW, px) * N;
-    if (blocks > 0x7fffffffll) return HIFIC_ERR_UNSUPPORTED;
-    p.tiles = (unsigned)cdivl(p.HW, px);
-    const dim3 grid((unsigned)blocks);
-    if (px == 1) hipLaunchKernelGGL((norm8_fwd_kernel<T, MODE, FMT, 1>), grid, dim3(256), 0, st, p);
-    else if (px == 16) hipLaunchKernelGGL((norm8_fwd_kernel<T, MODE, FMT, 16>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((norm8_fwd_kernel<T, MODE, FMT, 64>), grid, dim3(256), 0, st, p);
+    const int px = any_px(N, p.C, p.HW);
+    const long long tokens = (long long)N * p.HW;
+    const dim3 grid(any_grid(cdivl(tokens, px)));
+    if (px == 1) hipLaunchKernelGGL((norm8_fwd_kernel<T, MODE, FMT, 1>), grid, dim3(256), 0, st, p, tokens);
+    else if (px == 16) hipLaunchKernelGGL((norm8_fwd_kernel<T, MODE, FMT, 16>), grid, dim3(256), 0, st, p, tokens);
+    else hipLaunchKernelGGL((norm8_fwd_kernel<T, MODE, FMT, 64>), grid, dim3(256), 0, st, p, tokens);
     return hific_launch_status();
 }
 }  // namespace
@@ -359,6 +372,7 @@ int hific_rms_norm_fwd(const void* x, const void* resid, const float* w, void* y
     if (!x || !w || N <= 0 || C <= 0 || HW <= 0 || !act8_dtype_ok(dtype) || !(eps > 0.f)) return HIFIC_ERR_ARG;
     if ((resid != nullptr) != (h != nullptr) || (q != nullptr) != (qe != nullptr) || (!y && !q)) return HIFIC_ERR_ARG;
     if (q && !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
+    if (C > ACT8_MAX_C) return HIFIC_ERR_UNSUPPORTED;
     NormFwd p{x, resid, w, nullptr, y, h, rstd, (u8_t*)q, (u8_t*)qe, nullptr, nullptr, C, HW, 0, eps, 0, q_of_y, 0.f, 0.f};
 #define RMS(T) (!q ? norm8_fwd_launch<T, M_RMS, Q_NONE>(p, N, st) : fmt == HIFIC_Q_INT8                                     \
                    ? norm8_fwd_launch<T, M_RMS, HIFIC_Q_INT8>(p, N, st) : norm8_fwd_launch<T, M_RMS, HIFIC_Q_E4M3>(p, N, st))
@@ -371,6 +385,7 @@ int hific_channelnorm8_fwd(const void* x, const float* gamma, const float* beta,
     if (!x || !gamma || !beta || !y || !rstd || !q || !qe || N <= 0 || C < 2 || HW <= 0 || !(eps > 0.f)) return HIFIC_ERR_ARG;
     if (!act8_dtype_ok(dtype) || !act8_fmt_ok(fmt)) return HIFIC_ERR_ARG;
     if ((q2 != nullptr) != (qe2 != nullptr) || (q2 && !resid)) return HIFIC_ERR_ARG;
+    if (C > ACT8_MAX_C) return HIFIC_ERR_UNSUPPORTED;
     NormFwd p{x, resid, gamma, beta, y, nullptr, rstd, (u8_t*)q, (u8_t*)qe, (u8_t*)q2, (u8_t*)qe2, C, HW, 0, eps, relu, 0, 0.f, 0.f};
 #define CN(T) (fmt == HIFIC_Q_INT8 ? norm8_fwd_launch<T, M_CHAN, HIFIC_Q_INT8>(p, N, st) : norm8_fwd_launch<T, M_CHAN, HIFIC_Q_E4M3>(p, N, st))
     return dtype == HIFIC_F32 ? CN(float) : CN(bf16_t);

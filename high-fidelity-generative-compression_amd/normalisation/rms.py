@@ -1,7 +1,7 @@
 """RMSNorm2D: root-mean-square norm over the channel dim, beside ChannelNorm2D (no mean, no shift; no counterpart in the reference).
 
 One parameter `gamma` shaped (1, C, 1, 1).  `forward(x, resid)` with a residual adds it first and also returns the sum - the residual
-stream of a pre-norm block - in one kernel (csrc/norm8.hip)."""
+stream of a pre-norm block - in one kernel (csrc/norm8_fwd.hip)."""
 import torch
 import torch.nn as nn
 

@@ -161,3 +161,17 @@ def test_large_batches_go_in_slices(hific):
     assert act8._slices(4, 2 ** 29 + 7) == [(0, 3), (3, 4)]
     with pytest.raises(lib.HificError):
         act8._slices(1, 2 ** 31)
+
+
+def test_sizes_beyond_what_a_token_or_a_launch_may_have(hific):
+    from hific_amd import act8, lib, ops
+    p, wide = ctypes.c_void_p(4096), 2 ** 20 + 1
+    assert lib.raw("hific_act8_pack")(p, p, p, 0, 1, wide, 1, 0, None) == -4
+    assert lib.raw("hific_rms_norm_fwd")(p, None, p, p, None, p, None, None, 0, 0, 1, wide, 1, 1e-6, 0, None) == -4
+    assert lib.raw("hific_rms_norm_bwd")(p, None, None, 0, p, p, None, p, p, p, 0, 1, wide, 1, 0, p, 1 << 40, None) == -4
+    assert lib.raw("hific_channelnorm8_fwd")(p, p, p, None, p, p, p, p, None, None, 0, 1, wide, 4, 1e-3, 0, 0, None) == -4
+    assert lib.raw("hific_channelnorm8_bwd")(p, p, 0, p, p, p, p, p, p, p, 0, None, 0, 1, wide, 4, 0, 0, p, 1 << 40, None) == -4
+    assert lib.raw("hific_norm8_bwd_ws_bytes")(1, wide, 4) == 0
+    with pytest.raises(lib.HificError):
+        ops.checkpoint8(torch.empty(1, 1).expand(1, wide))
+    assert act8._nchw(torch.empty(1, 1).expand(1, wide - 1)) == (1, wide - 1, 1)

@@ -672,3 +672,69 @@ def test_a_tensor_beyond_32_bit_offsets(hific, dev):
     assert torch.equal(y[-3:], ops.rms_norm(tail, w))
     del y, x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("shape", [(2 ** 21 + 37, 1, 8), (2 ** 21 + 37, 8), (2 ** 21 + 37, 9, 1, 1), (2 ** 26 + 77, 2), (2 ** 25 + 77, 2, 2)])
+def test_more_tokens_than_one_launch_holds(hific, dev, shape):
+    """Parts of the batch (planes, rows) or rounds of a workgroup (other shapes): every token as in a small batch, and the channel sums
+    theirs.  A lane adds at most 2^21 / 512 tiles of eight values in a row, and a hundred terms follow: 33000 * 2^-24 of the terms' sum."""
+    from hific_amd import ops
+    n, m = shape[0], 4099
+    whole, rest = divmod(n, m)
+
+    def repeat(t):
+        return torch.cat([t.repeat((whole,) + (1,) * (t.dim() - 1)), t[:rest]])
+    base, dyb = (_rand((m,) + shape[1:], s, torch.bfloat16).to(dev) for s in (301, 302))
+    w = _chan(shape, 303).to(dev)
+    x, dy = repeat(base), repeat(dyb)
+    a, b = ops.checkpoint8(x), ops.checkpoint8(base)
+    assert torch.equal(a.q, repeat(b.q)) and torch.equal(a.e, repeat(b.e))
+    assert torch.equal(ops.restore8(a), repeat(ops.restore8(b)))
+    del a
+
+    def count(t):                                        # sums over the large batch from the small one's terms
+        return whole * t.sum(0) + t[:rest].sum(0)
+    over = tuple(range(2, len(shape)))
+    for kept in (None, "int8"):
+        outs = []
+        for xs, ds in ((base, dyb), (x, dy)):
+            xd, wd = xs.clone().requires_grad_(), w.clone().requires_grad_()
+            y = ops.rms_norm(xd, wd, fmt=kept)
+            outs.append((y.detach(),) + torch.autograd.grad(y, (xd, wd), ds))
+        (y0, dx0, _), (y1, dx1, dw1) = outs
+        assert torch.equal(y1, repeat(y0)) and torch.equal(dx1, repeat(dx0)), kept
+        xh = base.double() * torch.rsqrt(base.double().square().mean(1, keepdim=True) + 1e-6)
+        if kept:
+            y = ops.rms_norm(base.clone().requires_grad_(), w, fmt=kept)
+            code = y.grad_fn.saved_tensors
+            xh = O.values(code[0].cpu(), code[1].cpu()).to(dev)
+        terms = (dyb.double() * xh).sum(over) if over else dyb.double() * xh
+        size = (dyb.double() * xh).abs().sum(over) if over else (dyb.double() * xh).abs()
+        _close(dw1, count(terms).cpu(), 0.0, 33000 * 2.0 ** -24 * count(size).cpu(), f"dweight {kept}")
+    if shape[1] > 1:
+        outs = []
+        for xs, ds in ((base, dyb), (x, dy)):
+            xd = xs.clone().requires_grad_()
+            y, k = ops.channel_norm8(xd, w, w - 1, relu=True)
+            outs.append((y.detach(), k.q, k.e) + torch.autograd.grad(y, xd, ds))
+            del y, k
+        for i, (s, t) in enumerate(zip(*outs)):
+            assert torch.equal(t, repeat(s)), i
+    del x, dy, outs
+    torch.cuda.empty_cache()
+
+
+def test_blocks_check_the_norm_against_the_convolution(hific, dev):
+    from hific_amd import lib, ops
+    from hific_amd.network.layers import HipConv2d
+    from hific_amd.normalisation.channel import ChannelNorm2D
+    conv, norm = HipConv2d(8, 16, 3).to(dev), ChannelNorm2D(12).to(dev)
+    x = torch.zeros(1, 8, 10, 10, device=dev)
+    with pytest.raises(lib.HificError, match="gamma"):
+        ops.conv_norm8(x, None, conv, norm)
+    norm = ChannelNorm2D(16).to(dev)
+    for x8 in (ops.checkpoint8(x[:, :, :9]), x):
+        with pytest.raises(lib.HificError, match="x8"):
+            ops.conv_norm8(x, x8, conv, norm)
+    with pytest.raises(lib.HificError, match="resid"):
+        ops.conv_norm8(x, None, conv, norm, resid=x)
