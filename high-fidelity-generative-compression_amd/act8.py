@@ -637,7 +637,7 @@ def _slices(N, per_sample):
 @functools.lru_cache(maxsize=1024)
 def _wgrad8_ws_bytes(*shape):
     """Workspace of the kernel that reads the 8-bit tensor itself; 0 where restoring it for the natural-order kernels is faster."""
-    return int(lib.raw("hific_wgrad8_ws_bytes")(*shape[:10])) if lib.raw("hific_wgrad8_prefer")(*shape) else 0
+    return int(lib.raw("hific_wgrad8_ws_bytes")(*shape)) if lib.raw("hific_wgrad8_prefer")(*shape) else 0
 
 
 def _graph_ws(x, tr, geom, N, C, H, W, K, R, S, cd):

@@ -94,6 +94,7 @@ template <typename V> __device__ __forceinline__ void forget(V& r) { asm volatil
 // end, and its first values are then computed twice, with the same result.
 typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
 typedef u32x2_t u32x2_a1 __attribute__((aligned(1)));
+typedef u32x4_t u32x4_a1 __attribute__((aligned(1)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef f32x4_t f32x4_a4 __attribute__((aligned(4)));
 

@@ -45,7 +45,7 @@ SIGNATURES = {
     "hific_rms_norm_bwd": (I, [P, P, P, I] + [P] * 6 + [I] * 5 + [P, Z, P]),
     "hific_channelnorm8_fwd": (I, [P] * 10 + [I] * 4 + [F, I, I, P]),
     "hific_channelnorm8_bwd": (I, [P, P, I] + [P] * 7 + [I, P] + [I] * 6 + [P, Z, P]),
-    "hific_wgrad8_ws_bytes": (Z, [I] * 10),
+    "hific_wgrad8_ws_bytes": (Z, [I] * 11),
     "hific_wgrad8_prefer": (I, [I] * 11),
     "hific_wgrad8": (I, [I, P, P, I, P, P, I, P, P] + [I] * 14 + [P, Z, P]),
     "hific_act_bwd": (I, [P, P, P, L, F, I, P]),

@@ -174,9 +174,9 @@ int hific_channelnorm8_bwd(const void* q, const void* qe, int fmt, const float* 
 
 /* Weight gradient of nn.Conv2d (transposed 0: q [N, C, H, W] its input, dy [N, K, OH, OW], dw [K, C, R, S]) or nn.ConvTranspose2d
  * (transposed 1: pt = pl = its padding, dw [C, K, R, S]) from the input in 8 bits (values as hific_act8_restore, gamma / beta / relu
- * included) and a bfloat16 dy; csrc/wgrad8.hip.  For planes that the natural-order kernels of hific_conv2d_bwd_weight do not take:
- * hific_wgrad8_prefer says whether this form is the faster one; otherwise restore and call those.  ws: 16-byte aligned. */
-size_t hific_wgrad8_ws_bytes(int transposed, int N, int C, int H, int W, int K, int R, int S, int OH, int OW);
+ * included) and a bfloat16 dy; csrc/wgrad8.hip.  hific_wgrad8_prefer says whether this form is the faster one (odd planes, small
+ * products); otherwise restore and call hific_conv2d_bwd_weight.  ws: 16-byte aligned. */
+size_t hific_wgrad8_ws_bytes(int transposed, int N, int C, int H, int W, int K, int R, int S, int OH, int OW, int stride);
 int hific_wgrad8_prefer(int transposed, int N, int C, int H, int W, int K, int R, int S, int OH, int OW, int stride);
 int hific_wgrad8(int transposed, const void* q, const void* qe, int fmt, const float* gamma, const float* beta, int relu, const void* dy,
                  float* dw, int N, int C, int H, int W, int K, int R, int S, int OH, int OW, int stride, int pt, int pl, int pad_mode,

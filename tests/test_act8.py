@@ -134,8 +134,8 @@ def test_entry_points_refuse_bad_arguments(hific):
     assert cnb(p, p, 0, p, p, p, p, p, p, p, 0, None, 0, 1, 8, 4, 0, 0, p, 4, None) == -2
     assert lib.raw("hific_norm8_bwd_ws_bytes")(0, 8, 4) == 0
     wg = lib.raw("hific_wgrad8")
-    need = lib.raw("hific_wgrad8_ws_bytes")(0, 2, 8, 6, 6, 4, 3, 3, 6, 6)
-    assert need > 0 and lib.raw("hific_wgrad8_ws_bytes")(0, 2, 8, 6, 6, 0, 3, 3, 6, 6) == 0
+    need = lib.raw("hific_wgrad8_ws_bytes")(0, 2, 8, 6, 6, 4, 3, 3, 6, 6, 1)
+    assert need > 0 and lib.raw("hific_wgrad8_ws_bytes")(0, 2, 8, 6, 6, 0, 3, 3, 6, 6, 1) == 0
     ok = [0, p, p, 0, None, None, 0, p, p, 2, 8, 6, 6, 4, 3, 3, 6, 6, 1, 1, 1, 1, 0, p, need, None]
 
     def refuse(at, value):

@@ -399,7 +399,7 @@ def test_both_forms_of_the_weight_gradient(hific, dev, monkeypatch, transposed, 
     start = _rand((c, k, r, r) if transposed else (k, c, r, r), 77)
     sums = []
     for own in (True, False):
-        monkeypatch.setattr(act8, "_wgrad8_ws_bytes", lambda *s: int(lib.raw("hific_wgrad8_ws_bytes")(*s[:10])) if own else 0)
+        monkeypatch.setattr(act8, "_wgrad8_ws_bytes", lambda *s: int(lib.raw("hific_wgrad8_ws_bytes")(*s)) if own else 0)
         for acc in (0, 1):
             dw = start.to(dev).clone()
             act8._conv_wgrad8(a.tensors(), True, dy, dw, acc, geom, lib.HIFIC_BF16)
@@ -738,3 +738,53 @@ def test_blocks_check_the_norm_against_the_convolution(hific, dev):
             ops.conv_norm8(x, x8, conv, norm)
     with pytest.raises(lib.HificError, match="resid"):
         ops.conv_norm8(x, None, conv, norm, resid=x)
+
+
+@pytest.mark.parametrize("transposed,n,c,h,w,k,r,stride,reflect", [
+    (False, 2, 20, 9, 11, 24, 3, 1, False), (False, 2, 20, 9, 11, 24, 3, 1, True), (False, 1, 18, 21, 19, 33, 5, 2, True), (False, 3, 40, 17, 33, 8, 3, 2, False),
+    (False, 1, 70, 8, 5, 20, 3, 1, True), (False, 2, 9, 40, 50, 40, 7, 1, True), (False, 1, 16, 30, 31, 20, 3, 3, False), (False, 9, 2, 33, 64, 5, 1, 1, False),
+    (True, 2, 24, 9, 8, 40, 3, 2, False), (True, 1, 33, 7, 11, 20, 5, 2, False), (True, 2, 10, 5, 6, 12, 4, 3, False)])
+def test_weight_gradient_form_of_odd_planes(hific, dev, transposed, n, c, h, w, k, r, stride, reflect):
+    """The kernels that read the 8-bit tensor themselves, whatever the shape's rule says: values, and what an infinity of dy and a token
+    that is not finite reach - the taps of the formula that see them (through the pad's zeros too), no others.  Products are exact; a sum
+    of P positions per weight adds matrix instructions of 16 and at most 256 parts in a row."""
+    from hific_amd import act8, lib, ops
+    pad = r // 2
+    a = ops.checkpoint8(_rand((n, c, h, w), 401).to(dev), fmt="e4m3")
+    oh, ow = ((h - 1) * stride - 2 * pad + r + stride - 1, (w - 1) * stride - 2 * pad + r + stride - 1) if transposed else (
+        (h + 2 * pad - r) // stride + 1, (w + 2 * pad - r) // stride + 1)
+    dy = _rand((n, k, oh, ow), 402, torch.bfloat16)
+    shape = (c, k, r, r) if transposed else (k, c, r, r)
+    mode = lib.PAD_REFLECT if reflect else lib.PAD_ZERO
+
+    def own(act, d):
+        size = int(lib.raw("hific_wgrad8_ws_bytes")(int(transposed), n, c, h, w, k, r, r, oh, ow, stride))
+        assert size > 0
+        ws, dw, d = torch.empty(size, dtype=torch.uint8, device=dev), torch.empty(shape, device=dev), d.to(dev)
+        lib.call("hific_wgrad8", int(transposed), lib.ptr(act.q), lib.ptr(act.e), 1, None, None, 0, lib.ptr(d), lib.ptr(dw), n, c, h, w, k, r, r, oh,
+                 ow, stride, pad, pad, mode, 0, lib.ptr(ws), size, lib.stream())
+        torch.cuda.synchronize()
+        return dw.cpu()
+
+    def formula(xv, dv):
+        x, d = (dv, xv) if transposed else (xv, dv)          # x is padded and has the taps
+        xp = torch.nn.functional.pad(x, (pad,) * 4 if not transposed else (pad, pad + r + stride) * 2, mode="reflect" if reflect else "constant")
+        hh, ww = d.shape[2], d.shape[3]
+        out = torch.empty(shape, dtype=torch.float64)
+        for i in range(r):
+            for j in range(r):
+                t = xp[:, :, i:i + (hh - 1) * stride + 1:stride, j:j + (ww - 1) * stride + 1:stride]
+                out[:, :, i, j] = (d.transpose(0, 1).flatten(1) @ t.transpose(0, 1).flatten(1).t())
+        return out
+    x = _vals(a)
+    terms = n * h * w if transposed else n * oh * ow
+    _close(own(a, dy), formula(x, dy.double()), 0.0, (terms / 16 + 272) * 2.0 ** -24 * formula(x.abs(), dy.double().abs()) + 1e-30, "dw")
+    e = a.e.clone()
+    e[0, 0, w - 1] = 255                                     # a corner, so that some taps never see it
+    bad, xb, db = ops.Act8(a.q, e), x.clone(), dy.clone()
+    xb[0, :, 0, w - 1] = float("nan")
+    db[n - 1, 0, oh - 1, 0] = float("inf")
+    for act, d, xv, dv in ((bad, dy, xb, dy), (a, db, x, db)):
+        got, want = own(act, d), formula(xv, dv.double())
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+        assert torch.equal(got[torch.isinf(got)].double(), want[torch.isinf(want)])
