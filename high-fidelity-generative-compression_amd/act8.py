@@ -663,19 +663,19 @@ def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd, own_ws=False):
     xt = torch.float32 if cd == lib.HIFIC_F32 else torch.bfloat16
     flags = ops._is_f32(dy) << 1 if cd == lib.HIFIC_BF16 else 0
     tr, OH, OW = int(len(geom) == 3), dy.shape[2], dy.shape[3]
-    for lo, hi in _slices(N, max(C * H * W, K * OH * OW)):
-        d = c16(dy[lo:hi])
-        n = _wgrad8_ws_bytes(tr, hi - lo, C, H, W, K, R, S, OH, OW, geom[0]) if dy.dtype == torch.bfloat16 and cd == lib.HIFIC_BF16 else 0
+    small = max(C * H * W, K * OH * OW)
+    for lo, hi in ((0, N),) if N * small <= _MAX_ELEMENTS else _slices(N, small):
+        qs, es, d = (q, e, dy) if hi - lo == N else (q[lo:hi], e[lo:hi], c16(dy[lo:hi]))
+        n = _wgrad8_ws_bytes(tr, hi - lo, C, H, W, K, R, S, OH, OW, geom[0]) if dy.dtype is torch.bfloat16 and cd == lib.HIFIC_BF16 else 0
         if n:
             ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
             pt, pl, mode = (geom[1], geom[1], lib.PAD_ZERO) if tr else (geom[1], geom[2], geom[5])
-            lib.call("hific_wgrad8", tr, ptr(q[lo:hi]), ptr(e[lo:hi]), _CODE[q.dtype], ptr(gamma), ptr(beta), int(relu), ptr(d), ptr(dw),
-                     hi - lo, C, H, W, K, R, S, OH, OW, geom[0], pt, pl, mode, acc, ptr(ws), n, stream())
-            acc = 1
-            continue
-        x = _restore(q[lo:hi], e[lo:hi], gamma, beta, relu, xt)
-        ws = _graph_ws(x, tr, geom, hi - lo, C, H, W, K, R, S, cd) if own_ws else ops._ws(x)
-        lib.call(name, ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, *geom, acc, cd, flags, *ws, stream())
+            lib.call("hific_wgrad8", tr, qs.data_ptr(), es.data_ptr(), _CODE[q.dtype], ptr(gamma), ptr(beta), int(relu), d.data_ptr(),
+                     dw.data_ptr(), hi - lo, C, H, W, K, R, S, OH, OW, geom[0], pt, pl, mode, acc, ws.data_ptr(), n, stream())
+        else:
+            x = _restore(qs, es, gamma, beta, relu, xt)
+            ws = _graph_ws(x, tr, geom, hi - lo, C, H, W, K, R, S, cd) if own_ws else ops._ws(x)
+            lib.call(name, ptr(x), ptr(d), ptr(dw), hi - lo, C, H, W, K, R, S, *geom, acc, cd, flags, *ws, stream())
         acc = 1
 
 
