@@ -1,8 +1,10 @@
 // Activation checkpoints in 8 bits (format: act8.h): pack an activation, restore it.  Both are bound by HBM: pack reads T and
-// writes 1 byte per element, restore the reverse.
+// writes 1 byte per element, restore the reverse.  bfloat16, us (TB/s): 16x60x256x256 pack 39 (4.8), restore 40 (4.7); 16x240x64x64 9.6
+// (4.9) both; 16x960x16x16 4.8 (2.4) both, half of it the launch.
 #include "act8.h"
 
-// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor read twice (the second time from L2).
+// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor read twice (the second time from L2; 2x3000x32x32
+// float32 115 us, ten times what memory needs: a few workgroups with long chains of loads).
 template <typename T, int FMT, int PX>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                         int C, int HW, long long tokens) {
@@ -27,7 +29,8 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x,
     }
 }
 
-// Planes of eight positions and more: the tile stays in registers between the maximum and the rounding, one pass over HBM.
+// Planes of eight positions and more: the tile stays in registers between the maximum and the rounding, one pass over HBM (3x220x45x31
+// 3.7 us against a floor of 0.5: latency).
 template <typename T, int FMT, int LPX, int CPT>
 __global__ __launch_bounds__(256) void act8_pack_tile_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                              int C, int HW, unsigned tiles, unsigned blocks) {
@@ -114,7 +117,7 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const u8_t* __restric
     }
 }
 
-// Rows (HW = 1) of eight channels and more: eight channels per lane, L lanes and K groups per lane for a row.
+// Rows (HW = 1) of eight channels and more: eight channels per lane, L lanes and K groups per lane for a row (row_pick).
 template <typename T, int FMT, int L, int K>
 __global__ __launch_bounds__(row_block(L)) void act8_pack_rows_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe, int N, int C) {
     const int l = threadIdx.x % L;

@@ -1,4 +1,5 @@
-// norm8_fwd.hip, norm8_bwd.hip: norms that write or read activations in 8 bits (format: act8.h), and the root-mean-square norm.  Per token t of x [N, C, HW]:
+// norm8_fwd.hip, norm8_bwd.hip: norms that write or read activations in 8 bits (format: act8.h), and the root-mean-square norm.
+// Per token t of x [N, C, HW]:
 //   RMS norm      h = x (+ resid, rounded to the storage type: the new residual stream),  r = rsqrt(sum_c h^2 / C + eps),
 //                 xh = h r,  y = w_c xh
 //                 backward: g = w dy,  dx = r (g - xh sum_c(g xh) / C) (+ dstream),  dw_c = sum_t dy xh

@@ -27,7 +27,8 @@ struct WgTaps {
 // T, eight neighbours of one row (of eight and more) per thread, at the row's end moved back to end with it.  What they are read from
 // lies in one window of eight (stride 2: sixteen) bytes of one input row, reflected columns included: a byte permutation picks them,
 // and only the lanes at a row's ends form its selectors.  Other shapes (narrow rows, large strides or pads), and the ends of bfloat16
-// rows: value by value.  (3x437x35x44, 3x3: 12 us with all rows' ends value by value.)
+// rows: value by value.  Bound by the latency of its index arithmetic and loads on small planes (2x120x61x47 stride 2: 5.5 us), by its
+// instructions on large ones (16x480x32x32 stride 2, 25 MB written: 17 us, value by value 41).
 template <int SRC>
 __global__ __launch_bounds__(256) void wgrad8_taps_kernel(const WgTaps p, bf16_t* __restrict__ out, unsigned total) {
     const unsigned idx = blockIdx.x * 256 + threadIdx.x;
@@ -160,8 +161,10 @@ struct WgGemm {
 // positions; a group stays in its image, the image's last one is moved back to end with it and the positions it repeats are set to
 // zero in both operands (zero times an infinity of one would be NaN).  TILE x TILE per workgroup, four waves as 2 x 2,
 // v_mfma_f32_32x32x16_bf16; both tiles of the next slice travel through registers into the other half of LDS while this one is
-// multiplied: one barrier per slice (two or four slices ahead in registers: 9 to 40 % slower).  Rows of 144 bytes: conflict-free 16-byte fragment reads.  The tiles of one split go to one XCD,
-// whose L2 then holds the split's part of both operands.
+// multiplied: one barrier per slice (two or four slices ahead in registers: 9 to 36 % slower).  Rows of 144 bytes: conflict-free 16-byte
+// fragment reads.  The tiles of one split go to one XCD, whose L2 then holds the split's part of both operands (4 to 6 %).
+// 3x437x35x44 to 793 channels, 3x3: 56 us, 515 TFLOP/s; 960 x 960 on 16x16x16: 134 us, 507.  By count a slice of the large tile takes 768
+// cycles of LDS against 512 of matrix instructions, and at 2-byte addresses about as many in the vector cache.
 template <int TILE>
 __global__ __launch_bounds__(256) void wgrad8_gemm_kernel(const WgGemm p) {
     constexpr int PITCH = 144, BYTES = TILE * PITCH, PIECES = TILE * 8 / 256, F = TILE / 64;      // F x F fragments per wave
