@@ -271,18 +271,19 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
     return (total & 7u) == 0 ? (bid & 7u) * (total >> 3) + (bid >> 3) : bid;
 }
 
-// Tile of the plane kernels: 256 threads, LPX groups of eight positions, 256 / LPX channel groups, at most `most` channels per
+// Tile of the plane kernels: NW waves, LPX groups of eight positions, 64 NW / LPX channel groups, at most `most` channels per
 // thread, images of less than 4 GiB.  The widest LPX that fits the channels (what a tile costs besides its values - reductions,
 // scales, barriers - is shared by most values then: norm forward 16x60x256x256 75 us, with LPX <= 8 120), then narrower while
 // there are CUs without a workgroup (16x960x16x16: 256 wide tiles 12 us, 512 narrow ones 13.4) or more than an eighth of the lanes
-// lies past the planes' ends.  lpx = 0: more channels than the
-// registers hold, or images beyond 32-bit byte offsets.
-struct TileCfg { int lpx, cpt; unsigned tiles; long long blocks; };      // (tiles per image, less than 2^20; of the batch)
-static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
-    TileCfg t{0, 0, 0, 0};
-    if ((long long)(C + 256) * HW > (1ll << 30) - 64) return t;      // (C + 256: a lane's offset is formed before it is dropped)
-    for (int lpx = 32; lpx >= 1; lpx >>= 1) {
-        const int cpt = cdiv(C, 256 / lpx);
+// lies past the planes' ends.  Eight waves in the place of four where four would read less than 128 bytes of a channel at a time
+// (four / eight waves, norm forward 4x550x50x68 24 / 16 us, 16x480x64x64 47 / 43, backward 63 / 49; 16x960x16x16 9.3 / 8.6, backward
+// 14 / 12; eight for 16x240x64x64 too: forward 16.9 / 16.3, backward 24 / 28).
+// lpx = 0: more channels than the registers hold, or images beyond 32-bit byte offsets.
+struct TileCfg { int lpx, cpt, nw; unsigned tiles; long long blocks; };  // (tiles per image, less than 2^20; of the batch)
+static inline TileCfg tile_waves(long long N, int C, int HW, int most, int nw) {
+    TileCfg t{0, 0, nw, 0, 0};
+    for (int lpx = nw == 4 ? 32 : 8; lpx >= 1; lpx >>= 1) {
+        const int cpt = cdiv(C, 64 * nw / lpx);
         if (cpt > most) continue;
         t.lpx = lpx; t.cpt = cpt;
         t.tiles = (unsigned)cdiv(cdiv(HW, 8), lpx);
@@ -292,15 +293,35 @@ static inline TileCfg tile_pick(long long N, int C, int HW, int most) {
     }
     return t;
 }
-// F(LPX, CPT) for the configuration t
+static inline TileCfg tile_pick(long long N, int C, int HW, int most, int bytes) {
+    if ((long long)(C + 512) * HW > (1ll << 30) - 64) return TileCfg{0, 0, 4, 0, 0};     // (C + 512: a lane's offset is formed before it is dropped)
+    const TileCfg t = tile_waves(N, C, HW, most, 4);
+    return t.lpx == 0 || (t.lpx * 8 * bytes < 128 && C > 32 * most) ? tile_waves(N, C, HW, most, 8) : t;
+}
+// F(LPX, CPT, NW) for the configuration t
 #define TILE_DISPATCH(t, MOST, F)                                                                                         \
     do {                                                                                                                  \
-        if ((t).lpx == 32) { TILE_CPT(32, t, MOST, F); } else if ((t).lpx == 16) { TILE_CPT(16, t, MOST, F); }            \
-        else if ((t).lpx == 8) { TILE_CPT(8, t, MOST, F); } else if ((t).lpx == 4) { TILE_CPT(4, t, MOST, F); }           \
-        else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F); } else { TILE_CPT(1, t, MOST, F); }                             \
+        if ((t).nw == 8) {                                                                                                \
+            if ((t).lpx == 8) { TILE_CPT(8, t, MOST, F, 8); } else if ((t).lpx == 4) { TILE_CPT(4, t, MOST, F, 8); }      \
+            else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F, 8); } else { TILE_CPT(1, t, MOST, F, 8); }                   \
+        } else if ((t).lpx == 32) { TILE_CPT(32, t, MOST, F, 4); } else if ((t).lpx == 16) { TILE_CPT(16, t, MOST, F, 4); } \
+        else if ((t).lpx == 8) { TILE_CPT(8, t, MOST, F, 4); } else if ((t).lpx == 4) { TILE_CPT(4, t, MOST, F, 4); }     \
+        else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F, 4); } else { TILE_CPT(1, t, MOST, F, 4); }                       \
     } while (0)
-#define TILE_CPT(LPX, t, MOST, F)                                                                                         \
-    if ((t).cpt <= 1) { F(LPX, 1); } else if ((t).cpt <= 2) { F(LPX, 2); } else if ((t).cpt <= 4) { F(LPX, 4); } else { F(LPX, ((MOST) < 8 ? 4 : 8)); }
+#define TILE_CPT(LPX, t, MOST, F, NW)                                                                                     \
+    if ((t).cpt <= 1) { F(LPX, 1, NW); } else if ((t).cpt <= 2) { F(LPX, 2, NW); } else if ((t).cpt <= 4) { F(LPX, 4, NW); } \
+    else { F(LPX, ((MOST) < 8 ? 4 : 8), NW); }
+// sum / maximum over the waves' results of a tile position
+template <int NW, int TP> __device__ __forceinline__ float waves_sum(const float (*red)[TP], int i) {
+    float s = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    if constexpr (NW == 8) s += (red[4][i] + red[5][i]) + (red[6][i] + red[7][i]);
+    return s;
+}
+template <int NW, int TP> __device__ __forceinline__ float waves_max(const float (*red)[TP], int i) {
+    float m = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
+    if constexpr (NW == 8) m = fmaxf(m, fmaxf(fmaxf(red[4][i], red[5][i]), fmaxf(red[6][i], red[7][i])));
+    return m;
+}
 
 // Rows: L lanes and K groups of eight channels per lane hold a row, in workgroups of row_block(L) threads.  Sums and maxima over the
 // row's L lanes, through LDS where a row has the whole workgroup.

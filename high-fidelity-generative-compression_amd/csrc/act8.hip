@@ -4,7 +4,7 @@
 #include "act8.h"
 
 // Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor read twice (the second time from L2; 2x3000x32x32
-// float32 115 us, ten times what memory needs: a few workgroups with long chains of loads).
+// 115 us, which the tiles below take in 10: a few workgroups with long chains of loads).
 template <typename T, int FMT, int PX>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                         int C, int HW, long long tokens) {
@@ -31,11 +31,11 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x,
 
 // Planes of eight positions and more: the tile stays in registers between the maximum and the rounding, one pass over HBM (3x220x45x31
 // 3.7 us against a floor of 0.5: latency).
-template <typename T, int FMT, int LPX, int CPT>
-__global__ __launch_bounds__(256) void act8_pack_tile_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
+template <typename T, int FMT, int LPX, int CPT, int NW>
+__global__ __launch_bounds__(64 * NW) void act8_pack_tile_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                              int C, int HW, unsigned tiles, unsigned blocks) {
-    constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
-    __shared__ unsigned red[4][TP];
+    constexpr int SUBS = 64 / LPX, G = NW * SUBS, TP = LPX * 8;
+    __shared__ unsigned red[NW][TP];
     __shared__ float inv_s[TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
     const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / tiles, tile = bid - n * tiles;
@@ -60,7 +60,10 @@ __global__ __launch_bounds__(256) void act8_pack_tile_kernel(const T* __restrict
     tile_reduce<LPX, true>(am, red[wave]);
     __syncthreads();
     if (tid < TP) {                      // (TP <= 256)
-        const unsigned code = q8_code<FMT>(umax(umax(red[0][tid], red[1][tid]), umax(red[2][tid], red[3][tid])));
+        unsigned m = red[0][tid];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) m = umax(m, red[i][tid]);
+        const unsigned code = q8_code<FMT>(m);
         inv_s[tid] = q8_inv_scale(code);
         const unsigned o = tile * LPX + (tid >> 3);
         if (o < octs) qe[(size_t)n * HW + umin(o * 8, (unsigned)HW - 8) + (tid & 7)] = (u8_t)code;
@@ -173,12 +176,12 @@ namespace {
 template <typename T, int FMT>
 int pack_launch(const T* x, u8_t* q, u8_t* qe, int N, int C, int HW, hipStream_t st) {
     if (HW >= 8) {
-        const TileCfg t = tile_pick(N, C, HW, 8);
+        const TileCfg t = tile_pick(N, C, HW, 8, sizeof(T));
         if (t.lpx) {
             return batch_parts(N, t.tiles, [&](long long n0, long long n) {
                 const long long at = n0 * C * HW;
                 const unsigned blocks = (unsigned)(t.tiles * n);
-#define TILE(LPX, CPT) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT>), dim3(blocks), dim3(256), 0, st, x + at, q + at, qe + n0 * HW, C, HW, t.tiles, blocks)
+#define TILE(LPX, CPT, NW) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT, NW>), dim3(blocks), dim3(64 * NW), 0, st, x + at, q + at, qe + n0 * HW, C, HW, t.tiles, blocks)
                 TILE_DISPATCH(t, 8, TILE);
 #undef TILE
                 return hific_launch_status();

@@ -83,13 +83,13 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
 
 // Planes: as norm8_fwd_tile_kernel.  A workgroup takes `pit` tiles in turn (p.tokens counts tiles here) and keeps the sums of its
 // channels in registers: part[workgroup][0..2][c] as norm8_param_kernel.  Bound by the issue of its instructions as much as by HBM (about
-// 20 per value: two unpackings, mask, two sums, three channel sums; registers allow two workgroups per CU).  bfloat16, us (TB/s): channel
-// norm + ReLU from int8 16x60x256x256 80 (3.9), 16x120x128x128 37 (4.2), 16x960x16x16 10 (2.0); root-mean-square norm with the stream's
-// gradient 114 (4.4), 55 (4.6), 11 (2.9).
-template <typename T, int MODE, int SRC, int LPX, int CPT>
-__global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
-    constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
-    __shared__ float red[2][4][TP], st[2][TP];
+// 20 per value: two unpackings, mask, two sums, three channel sums; registers allow eight waves per CU).  bfloat16, us (TB/s): channel
+// norm + ReLU from int8 16x60x256x256 80 (3.9), 16x120x128x128 37 (4.2), 16x960x16x16 8.5 (2.3); root-mean-square norm with the stream's
+// gradient 114 (4.4), 55 (4.6), 9.5 (3.3).
+template <typename T, int MODE, int SRC, int LPX, int CPT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
+    constexpr int SUBS = 64 / LPX, G = NW * SUBS, TP = LPX * 8;
+    __shared__ float red[2][NW][TP], st[2][TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
     const unsigned bid = xcd_block(blockIdx.x, blocks);
     const unsigned octs = ((unsigned)p.HW + 7) >> 3;
@@ -161,8 +161,8 @@ __global__ __launch_bounds__(256, 2) void norm8_bwd_tile_kernel(const NormBwd p,
         if (MODE == M_CHAN) tile_reduce<LPX, false>(s1, red[0][wave]);
         __syncthreads();
         if (tid < TP) {
-            st[1][tid] = ((red[1][0][tid] + red[1][1][tid]) + (red[1][2][tid] + red[1][3][tid])) * p.rv;
-            if (MODE == M_CHAN) st[0][tid] = ((red[0][0][tid] + red[0][1][tid]) + (red[0][2][tid] + red[0][3][tid])) * p.rc;
+            st[1][tid] = waves_sum<NW, TP>(red[1], tid) * p.rv;
+            if (MODE == M_CHAN) st[0][tid] = waves_sum<NW, TP>(red[0], tid) * p.rc;
         }
         __syncthreads();
 #pragma unroll
@@ -344,13 +344,17 @@ int norm8_nsplit(int N, int C, int HW) {                             // ~1024 wo
     return (int)(s < 1 ? 1 : s);
 }
 // tiles per workgroup of the backward plane kernel: 512 workgroups, two per CU (what its registers allow), each with its share of
-// the tiles - one round, few rows of channel sums (16x120x128x128: 43 us, with 1024 workgroups 47.5, with 2048 53)
-unsigned norm8_pit(const TileCfg& t) { return (unsigned)(t.blocks < 512 ? 1 : cdivl(t.blocks, 512)); }
+// the tiles - one round, few rows of channel sums (16x120x128x128: 43 us, with 1024 workgroups 47.5, with 2048 53); 256 of eight waves
+// (16x480x64x64: 49 us, 512 51)
+unsigned norm8_pit(const TileCfg& t) {
+    const int most = t.nw == 8 ? 256 : 512;
+    return (unsigned)(t.blocks < most ? 1 : cdivl(t.blocks, most));
+}
 // rows of channel sums that the backward pass writes
 template <typename T>
 size_t norm8_rows(int mode, int N, int C, int HW) {
     if (HW >= 8) {
-        const TileCfg t = tile_pick(N, C, HW, tile_most<T>());
+        const TileCfg t = tile_pick(N, C, HW, tile_most<T>(), sizeof(T));
         if (t.lpx) return (size_t)cdivl(t.blocks, norm8_pit(t));
     }
     if (mode == M_RMS && HW == 1 && C >= 8) {
@@ -370,16 +374,16 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
     const int nr = MODE == M_RMS ? 1 : 2 + p.db;
     const size_t rows = norm8_rows<T>(MODE, N, p.C, p.HW);
     if (rows * nr * p.C * sizeof(float) > ws_bytes) return HIFIC_ERR_WS;
-    TileCfg t{0, 0, 0, 0};
+    TileCfg t{0, 0, 4, 0, 0};
     RowCfg r{0, 0};
-    if (p.HW >= 8) t = tile_pick(N, p.C, p.HW, tile_most<T>());
+    if (p.HW >= 8) t = tile_pick(N, p.C, p.HW, tile_most<T>(), sizeof(T));
     else if (MODE == M_RMS && p.HW == 1 && p.C >= 8) r = row_pick(N, p.C);
     if (rows > 0x7fffffffull) return HIFIC_ERR_UNSUPPORTED;
     if (t.lpx) {
         p.tiles = t.tiles;
         const unsigned pit = norm8_pit(t);
         p.tokens = t.blocks;
-#define BWD(LPX, CPT) hipLaunchKernelGGL((norm8_bwd_tile_kernel<T, MODE, SRC, LPX, CPT>), dim3((unsigned)rows), dim3(256), 0, st, p, (unsigned)rows, pit)
+#define BWD(LPX, CPT, NW) hipLaunchKernelGGL((norm8_bwd_tile_kernel<T, MODE, SRC, LPX, CPT, NW>), dim3((unsigned)rows), dim3(64 * NW), 0, st, p, (unsigned)rows, pit)
         TILE_DISPATCH(t, tile_most<T>(), BWD);
 #undef BWD
     } else if (r.l) {

@@ -9,7 +9,8 @@ struct NormFwd {
     float rc, rv;                        // 1 / C, and 1 / C or 1 / (C - 1): a product in the place of a division per position
 };
 
-// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2; 2x3000x32x32 250 us).
+// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2; 2x3000x32x32 250 us, which
+// the tiles below take in 17).
 template <typename T, int MODE, int FMT, int PX>
 __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long long tokens) {
     constexpr int G = 256 / PX;
@@ -87,13 +88,13 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
 
 // Planes of eight positions and more: a workgroup owns LPX * 8 positions x all channels (tile_pick), eight positions and CPT
 // channels per lane, kept as they were loaded between the passes: every tensor crosses HBM once, and that bounds it.  bfloat16, us (TB/s): channel
-// norm + ReLU 16x60x256x256 70 (4.5), 16x120x128x128 38 (4.1), 16x960x16x16 9.2 (2.1: two tiles' latency); root-mean-square norm with
-// residual 105 (4.8), 56 (4.5), 8.8 (3.6).
-template <typename T, int MODE, int FMT, bool RES, int LPX, int CPT>
-__global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p, unsigned blocks) {
-    constexpr int SUBS = 64 / LPX, G = 4 * SUBS, TP = LPX * 8;
+// norm + ReLU 16x60x256x256 70 (4.5), 16x120x128x128 38 (4.1), 16x960x16x16 8.6 (2.3: the latency of three dependent passes);
+// root-mean-square norm with residual 105 (4.8), 56 (4.5), 8.5 (3.7).
+template <typename T, int MODE, int FMT, bool RES, int LPX, int CPT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFwd p, unsigned blocks) {
+    constexpr int SUBS = 64 / LPX, G = NW * SUBS, TP = LPX * 8;
     constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;
-    __shared__ float red[4][TP], redm[4][TP];
+    __shared__ float red[NW][TP], redm[NW][TP];
     __shared__ float st_r[TP], st_inv[TP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pl = lane % LPX, g = wave * SUBS + lane / LPX;
     const unsigned bid = xcd_block(blockIdx.x, blocks), n = bid / p.tiles, tile = bid - n * p.tiles;
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
                 for (int j = 0; j < 8; ++j) acc[j] += xr[k].get(j);
         tile_reduce<LPX, false>(acc, red[wave]);
         __syncthreads();
-        if (tid < TP) st_r[tid] = ((red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid])) * p.rc;
+        if (tid < TP) st_r[tid] = waves_sum<NW, TP>(red, tid) * p.rc;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; ++j) { mu[j] = st_r[pl * 8 + j]; acc[j] = 0.f; }
@@ -163,13 +164,13 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
     if (FMT != Q_NONE) tile_reduce<LPX, true>(am, redm[wave]);
     __syncthreads();
     if (tid < TP) {
-        const float ss = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+        const float ss = waves_sum<NW, TP>(red, tid);
         const float r = rsqrtf(ss * p.rv + p.eps);
         st_r[tid] = r;
         if (p.rstd && sok) p.rstd[stok] = r;
         if (FMT != Q_NONE) {
             // max|d| r = max|d r|: a rounded product is monotone (with q_of_y the weight comes between, and q8_pack8 clamps)
-            const float m = fmaxf(fmaxf(redm[0][tid], redm[1][tid]), fmaxf(redm[2][tid], redm[3][tid]));
+            const float m = waves_max<NW, TP>(redm, tid);
             const unsigned code = q8_code<F>(abs_bits(m * r));
             st_inv[tid] = q8_inv_scale(code);
             if (sok) p.qe[stok] = (u8_t)code;
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void norm8_fwd_tile_kernel(const NormFwd p,
         tile_reduce<LPX, true>(am, redm[wave]);          // (a NaN as an infinity; redm's readers are behind a barrier)
         __syncthreads();
         if (tid < TP) {
-            const unsigned code = q8_code<F>(abs_bits(fmaxf(fmaxf(redm[0][tid], redm[1][tid]), fmaxf(redm[2][tid], redm[3][tid]))));
+            const unsigned code = q8_code<F>(abs_bits(waves_max<NW, TP>(redm, tid)));
             st_inv[tid] = q8_inv_scale(code);
             if (sok) p.qe2[stok] = (u8_t)code;
         }
@@ -329,16 +330,16 @@ int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
     p.rc = 1.f / (float)p.C;
     p.rv = 1.f / (float)(MODE == M_RMS ? p.C : p.C - 1);
     if (p.HW >= 8) {
-        const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>());
+        const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>(), sizeof(T));
         if (t.lpx) {
             p.tiles = t.tiles;
             return batch_parts(N, t.tiles, [&](long long n0, long long n) {
                 const NormFwd part = norm8_part<T>(p, n0);
                 const dim3 grid((unsigned)(t.tiles * n));
-#define FWD(LPX, CPT)                                                                                                               \
+#define FWD(LPX, CPT, NW)                                                                                                           \
                 do {                                                                                                                \
-                    if (p.resid) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, true, LPX, CPT>), grid, dim3(256), 0, st, part, grid.x); \
-                    else hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, false, LPX, CPT>), grid, dim3(256), 0, st, part, grid.x); \
+                    if (p.resid) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, true, LPX, CPT, NW>), grid, dim3(64 * NW), 0, st, part, grid.x); \
+                    else hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, false, LPX, CPT, NW>), grid, dim3(64 * NW), 0, st, part, grid.x); \
                 } while (0)
                 TILE_DISPATCH(t, tile_most<T>(), FWD);
 #undef FWD

@@ -788,3 +788,18 @@ def test_weight_gradient_form_of_odd_planes(hific, dev, transposed, n, c, h, w, 
         got, want = own(act, d), formula(xv, dv.double())
         assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
         assert torch.equal(got[torch.isinf(got)].double(), want[torch.isinf(want)])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 300, 7, 9), (1, 515, 5, 7), (3, 700, 9, 9), (1, 1100, 2, 4), (2, 513, 33, 16), (1, 2900, 5, 5), (1, 4096, 3, 3), (1, 4100, 2, 5)])
+def test_planes_of_many_channels(hific, dev, shape, dt):
+    """The tests above at the widths where a tile takes more waves, or none holds it."""
+    for fmt in ("int8", "e4m3"):
+        test_checkpoint_is_the_oracles_bit_for_bit(hific, dev, shape, dt, fmt)
+        test_rms_norm8(hific, dev, shape, dt, True, fmt)
+        for relu, resid in ((True, False), (False, True)):
+            test_channel_norm8(hific, dev, shape, dt, relu, resid, fmt)
+    for resid in (False, True):
+        test_rms_norm_forward(hific, dev, shape, dt, resid)
+        test_rms_norm_backward(hific, dev, shape, dt, resid, None)
+    test_rms_norm_backward(hific, dev, shape, dt, True, "int8")
