@@ -277,10 +277,12 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
 // there are CUs without a workgroup (16x960x16x16: 256 wide tiles 12 us, 512 narrow ones 13.4) or more than an eighth of the lanes
 // lies past the planes' ends.  Eight waves in the place of four where four would read less than 128 bytes of a channel at a time
 // (four / eight waves, norm forward 4x550x50x68 24 / 16 us, 16x480x64x64 47 / 43, backward 63 / 49; 16x960x16x16 9.3 / 8.6, backward
-// 14 / 12; eight for 16x240x64x64 too: forward 16.9 / 16.3, backward 24 / 28).
+// 14 / 12; eight for 16x240x64x64 too: forward 16.9 / 16.3, backward 24 / 28), and fewer workgroups of
+// those are enough before pieces of 16 or 32 bytes are (bfloat16 15x909x22x8: 330 of LPX 1 13.9 us, 165 of LPX 2 9.8; 13x336x50x8: 325 of
+// LPX 2 8.4, 169 of LPX 4 7.0; but 16x960x16x16: 256 of LPX 2 8.6, 128 of LPX 4 9.4).
 // lpx = 0: more channels than the registers hold, or images beyond 32-bit byte offsets.
 struct TileCfg { int lpx, cpt, nw; unsigned tiles; long long blocks; };  // (tiles per image, less than 2^20; of the batch)
-static inline TileCfg tile_waves(long long N, int C, int HW, int most, int nw) {
+static inline TileCfg tile_waves(long long N, int C, int HW, int most, int bytes, int nw) {
     TileCfg t{0, 0, nw, 0, 0};
     for (int lpx = nw == 4 ? 32 : 8; lpx >= 1; lpx >>= 1) {
         const int cpt = cdiv(C, 64 * nw / lpx);
@@ -289,14 +291,15 @@ static inline TileCfg tile_waves(long long N, int C, int HW, int most, int nw) {
         t.tiles = (unsigned)cdiv(cdiv(HW, 8), lpx);
         t.blocks = (long long)t.tiles * N;
         const long long octs = cdiv(HW, 8);
-        if ((t.blocks >= 256 || cpt <= 1) && (lpx == 1 || (long long)t.tiles * lpx * 8 <= octs * 9)) break;
+        const int enough = nw == 4 ? 256 : (lpx * 8 * bytes > 32 ? 150 : 100);
+        if ((t.blocks >= enough || cpt <= 1) && (lpx == 1 || (long long)t.tiles * lpx * 8 <= octs * 9)) break;
     }
     return t;
 }
 static inline TileCfg tile_pick(long long N, int C, int HW, int most, int bytes) {
     if ((long long)(C + 512) * HW > (1ll << 30) - 64) return TileCfg{0, 0, 4, 0, 0};     // (C + 512: a lane's offset is formed before it is dropped)
-    const TileCfg t = tile_waves(N, C, HW, most, 4);
-    return t.lpx == 0 || (t.lpx * 8 * bytes < 128 && C > 32 * most) ? tile_waves(N, C, HW, most, 8) : t;
+    const TileCfg t = tile_waves(N, C, HW, most, bytes, 4);
+    return t.lpx == 0 || (t.lpx * 8 * bytes < 128 && C > 32 * most) ? tile_waves(N, C, HW, most, bytes, 8) : t;
 }
 // F(LPX, CPT, NW) for the configuration t
 #define TILE_DISPATCH(t, MOST, F)                                                                                         \
