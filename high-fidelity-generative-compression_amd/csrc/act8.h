@@ -175,9 +175,8 @@ __device__ __forceinline__ void q8_scales(u32x2_t e, float* scale, float* s128) 
     }
 }
 
-// eight normalised values of a channel whose ReLU follows, as x = xh / scale, v = fma(gs, x, beta) with gs = gamma * scale (the
-// same product as gamma * xh): q8_round_masked of each, and v
-// becomes relu(v).  No clamp: max|xh| gave the exponent, so |x| <= QMAX, and the neighbour
+// eight normalised values of a channel whose ReLU follows, as x = xh / scale, with v = fma(gamma, xh, beta) and gs = gamma * scale:
+// q8_round_masked of each, and v becomes relu(v).  No clamp: max|xh| gave the exponent, so |x| <= QMAX, and the neighbour
 // that is taken lies between x and the nearest value's other side.
 template <int FMT>
 __device__ __forceinline__ u32x2_t q8_pack8_masked(const float* x, float* v, const float* gs, float beta, float gamma) {

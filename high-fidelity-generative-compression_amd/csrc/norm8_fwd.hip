@@ -177,45 +177,32 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
         }
     }
     __syncthreads();
-    // x = d * (r / scale) is xh / scale: dividing by a power of two commutes with the rounding, and so does gs below
-    float r[8], ri[8];
+    // (xh / scale in two products: r / scale overflows where a token's values are all alike or nearly so)
+    float r[8], inv[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float inv = FMT != Q_NONE ? st_inv[pl * 8 + j] : 0.f;
-        r[j] = st_r[pl * 8 + j]; ri[j] = r[j] * inv; am[j] = 0.f;
-        // behind a ReLU only x and gs are formed: r's place holds the scale 1 / inv, a power of two (2^127 for a token that is not
-        // finite: its values are NaN)
-        if (MODE == M_CHAN && FMT != Q_NONE && p.relu) r[j] = __uint_as_float(0x7f000000u - __float_as_uint(inv));
-    }
+    for (int j = 0; j < 8; ++j) { r[j] = st_r[pl * 8 + j]; inv[j] = FMT != Q_NONE ? st_inv[pl * 8 + j] : 0.f; am[j] = 0.f; }
 #pragma unroll
     for (int k = 0; k < CPT; ++k) {
         const int c = g + G * k;
         if (c >= p.C) continue;
-        float o[8];
-        if (MODE == M_CHAN && FMT != Q_NONE && p.relu) {
-            float x[8], gs[8];
+        float o[8], xh[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                gs[j] = w[k] * r[j];
-                x[j] = (xr[k].get(j) - mu[j]) * ri[j];
-                o[j] = fmaf(gs[j], x[j], b[MODE == M_CHAN ? k : 0]);
-            }
-            const u32x2_t q = q8_pack8_masked<F>(x, o, gs, b[MODE == M_CHAN ? k : 0], w[k]);
+        for (int j = 0; j < 8; ++j) {
+            xh[j] = (xr[k].get(j) - mu[j]) * r[j];
+            o[j] = MODE == M_RMS ? xh[j] * w[k] : fmaf(w[k], xh[j], b[MODE == M_CHAN ? k : 0]);
+        }
+        if constexpr (FMT != Q_NONE) {
+            float t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = (MODE == M_RMS && p.q_of_y ? o[j] : xh[j]) * inv[j];
+            u32x2_t q;
+            if (MODE == M_CHAN && p.relu) {
+                float gs[8];             // gamma * scale; the scale 1 / inv is a power of two (2^127 for a token that is not finite: its values are NaN)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) gs[j] = w[k] * __uint_as_float(0x7f000000u - __float_as_uint(inv[j]));
+                q = q8_pack8_masked<F>(t, o, gs, b[MODE == M_CHAN ? k : 0], w[k]);
+            } else q = q8_pack8<F, MODE == M_RMS>(t);
             if (ok) *(u32x2_a1*)at(p.q + img, off + k * kst) = q;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float xh = (xr[k].get(j) - mu[j]) * r[j];
-                o[j] = MODE == M_RMS ? xh * w[k] : fmaf(w[k], xh, b[MODE == M_CHAN ? k : 0]);
-            }
-            if constexpr (FMT != Q_NONE) {
-                float t[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    t[j] = MODE == M_RMS && p.q_of_y ? o[j] * st_inv[pl * 8 + j] : (xr[k].get(j) - mu[j]) * ri[j];
-                const u32x2_t q = q8_pack8<F, MODE == M_RMS>(t);
-                if (ok) *(u32x2_a1*)at(p.q + img, off + k * kst) = q;
-            }
         }
         if constexpr (MODE == M_CHAN) {
             if constexpr (RES) {         // both terms rounded to the storage type first, as norm and add one after the other

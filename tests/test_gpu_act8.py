@@ -803,3 +803,56 @@ def test_planes_of_many_channels(hific, dev, shape, dt):
         test_rms_norm_forward(hific, dev, shape, dt, resid)
         test_rms_norm_backward(hific, dev, shape, dt, resid, None)
     test_rms_norm_backward(hific, dev, shape, dt, True, "int8")
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 2, 24, 20), (3, 60, 8, 8), (1, 960, 16, 16), (2, 300, 7, 9), (2, 33, 2, 3), (1, 4100, 2, 5), (9, 40), (5, 3000), (6, 5)])
+def test_tokens_of_equal_values(hific, dev, shape, dt, fmt):
+    """Tokens without a deviation (a flat patch, zeros), and with one of the smallest numbers: normalised to nothing, never to NaN.  The
+    mean of equal values is a rounded sum times a rounded 1 / C, so it misses them by up to F32 of their size (the chains that F32
+    counts), and rsqrt(eps) multiplies that; of zeros and of the smallest numbers nothing is left at all."""
+    from hific_amd import ops
+    t = TYPES[dt]
+    x, w, b = _rand(shape, 501, t), _chan(shape, 502), _chan(shape, 503, 0.0)
+    flat = x.reshape(shape[0], shape[1], -1)
+    tiny = torch.where(torch.arange(shape[1]) % 2 == 0, 2.0 ** -125, -2.0 ** -125).to(t)
+    flat[0, :, 0], flat[-1, :, -1] = 0.0, 1.5
+    flat[shape[0] // 2, :, flat.shape[2] // 2] = tiny
+    alike = torch.zeros(flat[:, 0].shape, dtype=torch.bool)
+    alike[0, 0] = alike[-1, -1] = alike[shape[0] // 2, flat.shape[2] // 2] = True
+    dy, rs = _rand(shape, 504, t), _rand(shape, 505, t)
+
+    def at(v):
+        return v.detach().cpu().reshape(shape[0], shape[1], -1).transpose(1, 2)[alike].double()
+    miss = F32 * at(x).abs().amax(1, keepdim=True) / math.sqrt(1e-3)
+    for relu, resid in ((False, False), (True, False), (True, True), (False, True)):
+        leaves = [v.to(dev).requires_grad_() for v in (x, w, b)]
+        y, a = ops.channel_norm8(*leaves, relu=relu, resid=rs.to(dev) if resid else None, fmt=fmt)
+        q, e, rstd, _, _ = y.grad_fn.saved_tensors
+        kept = O.values(q.cpu(), e.cpu())
+        grads = torch.autograd.grad(y, leaves, dy.to(dev))
+        want = (torch.relu(b) if relu else b).double().expand(int(alike.sum()), -1)
+        if resid:
+            want = want.to(t).double() + at(rs)
+        # (two roundings to the type with a residual: the norm's value, which miss may move across a border, and the sum)
+        steps = _half(t) * want.abs() + (2 * _half(t) * (b.double().abs() + miss * w.double().abs()) if resid else 0.0)
+        assert ((at(y) - want).abs() <= steps + 1.01 * miss * w.double().abs() + 2.0 ** -110).all()
+        assert (at(kept).abs() <= 1.01 * miss + 2.0 ** -110).all() and torch.isfinite(kept).all()
+        assert torch.isfinite(ops.restore8(a, torch.float32)).all()
+        wdx, wdg, wdb = O.channel_norm_grad(kept, rstd.cpu().double().unsqueeze(1), w, b, dy, relu)
+        size = rstd.cpu().double().unsqueeze(1) * (dy.double() * O._ch(w, x)).abs().amax(1, keepdim=True) * (1 + kept.abs().amax(1, keepdim=True)) * 2
+        _close(grads[0], wdx, _half(t), F32 * size, "dx")
+        dims = [0] + list(range(2, x.dim()))
+        _close(grads[1], wdg, 0.0, 8 * F32 * (dy.double() * kept).abs().sum(dims) + 1e-30, "dgamma")
+    z = x.clone()
+    z.reshape(shape[0], shape[1], -1).transpose(1, 2)[alike] = 0
+    zd, wd = z.to(dev).requires_grad_(), w.to(dev).requires_grad_()
+    y = ops.rms_norm(zd, wd, fmt=fmt)
+    q, e, rstd, _ = y.grad_fn.saved_tensors
+    kept = O.values(q.cpu(), e.cpu())
+    assert (at(kept) == 0).all() and (at(y) == 0).all() and torch.isfinite(kept).all()
+    dx, _ = torch.autograd.grad(y, (zd, wd), dy.to(dev))
+    assert torch.isfinite(dx).all()
+    with torch.no_grad():
+        assert (at(ops.restore8(ops.rms_norm8(zd, wd, fmt=fmt), torch.float32)) == 0).all()
