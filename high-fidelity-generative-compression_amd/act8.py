@@ -204,10 +204,11 @@ def _bwd_ws_bytes(N, C, HW):
     return int(lib.raw("hific_norm8_bwd_ws_bytes")(N, C, HW))
 
 
-def _bwd_ws(N, C, HW, device):
-    # its own allocation per call, not the stream's workspace: two captured graphs that replay on two streams share nothing
+def _bwd_ws(N, C, HW, rstd):
+    # its own allocation per call (float32, like rstd), not the stream's workspace: two captured graphs that replay on two streams share
+    # nothing
     n = _bwd_ws_bytes(N, C, HW)
-    return torch.empty(n, dtype=torch.uint8, device=device), n
+    return rstd.new_empty(n >> 2), n
 
 
 class RmsNormFn(Function):
@@ -240,7 +241,7 @@ class RmsNormFn(Function):
         dx = torch.empty_like(dy)
         N, C, HW = ctx.geom
         if N and HW:
-            ws, n = _bwd_ws(N, C, HW, dy.device)
+            ws, n = _bwd_ws(N, C, HW, rstd)
             h, q = (kept.data_ptr(), None) if e is None else (None, kept.data_ptr())
             _launch("hific_rms_norm_bwd", dy, h, q, ptr(e), ctx.code, rstd.data_ptr(), dy.data_ptr(), ptr(dstream), weight.data_ptr(),
                     dx.data_ptr(), dwt.data_ptr(), acc, N, C, HW, ctx.cd, ws.data_ptr(), n)
@@ -304,11 +305,11 @@ def _cn8_fwd(x, gamma, beta, resid, eps, relu, geom, cd, code, dt):
     return y, rstd, q, e, q2, e2
 
 
-def _cn8_bwd(q, e, rstd, dy, gamma, beta, relu, dg, db, acc, dprev=None, acc_prev=0):
-    N, C, HW = _nchw(dy)
+def _cn8_bwd(q, e, rstd, dy, gamma, beta, relu, dg, db, acc, dprev=None, acc_prev=0, geom=None):
+    N, C, HW = geom or _nchw(dy)
     dx = torch.empty_like(dy)
     if N and HW:
-        ws, n = _bwd_ws(N, C, HW, dy.device)
+        ws, n = _bwd_ws(N, C, HW, rstd)
         _launch("hific_channelnorm8_bwd", dy, q.data_ptr(), e.data_ptr(), _CODE[q.dtype], rstd.data_ptr(), dy.data_ptr(), gamma.data_ptr(),
                 beta.data_ptr(), dx.data_ptr(), dg.data_ptr(), db.data_ptr(), acc, ptr(dprev), acc_prev, N, C, HW, int(relu),
                 lib.dtype_code(dy), ws.data_ptr(), n)
@@ -383,14 +384,14 @@ def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
     [N, ...] the reciprocal standard deviations, dy float32 or bfloat16."""
     if not isinstance(a, Act8) or a.gamma is not None:
         raise lib.HificError("channel_norm_grad8 needs the normalised values as an Act8 without gamma / beta")
-    _norm_args(a.q, gamma, beta, "channel_norm_grad8")
+    geom = _norm_args(a.q, gamma, beta, "channel_norm_grad8")
     if dy.shape != a.q.shape:
         raise lib.HificError(f"dy must be {tuple(a.shape)}, got {tuple(dy.shape)}")
     _one_device(a.q, dy, rstd)
     _param(rstd, a.e.numel(), "rstd")
     lib.dtype_code(dy)
     dg, db = torch.empty_like(gamma), torch.empty_like(beta)
-    return _cn8_bwd(a.q, a.e, rstd, c16(dy), gamma, beta, bool(relu), dg, db, 0), dg, db
+    return _cn8_bwd(a.q, a.e, rstd, c16(dy), gamma, beta, bool(relu), dg, db, 0, geom=geom), dg, db
 
 
 # ---- training with 8-bit checkpoints ---------------------------------------------------------------------------------------------
