@@ -146,17 +146,26 @@ __device__ __forceinline__ u32x2_t q8_pack8(const float* t) {
     }
     return o;
 }
-// eight bytes -> eight values, times scale[j] (s128 = -128 * scale for int8: bytes with the sign bit flipped convert in one
-// instruction, and (u - 128) * 2^e is exact in one fused multiply-add)
+// byte B of u, signed, as a number: one instruction (a sub-dword operand with sign extension; written out because the compiler extends
+// bytes that are used in two places in one of their own first: rows of 960 from int8, backward 65 us with it, 69 without)
+template <int B>
+__device__ __forceinline__ float byte_f32(unsigned u) {
+    float v;
+    if constexpr (B == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(v) : "v"(u));
+    else if constexpr (B == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(v) : "v"(u));
+    else if constexpr (B == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(v) : "v"(u));
+    else asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(v) : "v"(u));
+    return v;
+}
+// eight bytes -> eight values, times scale[j].  A product per value, whose result is the kept value whatever the scale (an offset
+// byte and one fused multiply-add would need 128 * scale, which is infinite from 2^121 on).
 template <int FMT>
-__device__ __forceinline__ void q8_unpack8(u32x2_t q, const float* scale, const float* s128, float* v) {
+__device__ __forceinline__ void q8_unpack8(u32x2_t q, const float* scale, float* v) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (FMT == HIFIC_Q_INT8) {
-            unsigned u = q[h] ^ 0x80808080u;
-            forget(u);                                           // (or the flip is undone and redone byte by byte)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * h + j] = fmaf((float)((u >> (8 * j)) & 0xffu), scale[4 * h + j], s128[4 * h + j]);
+            v[4 * h] = byte_f32<0>(q[h]) * scale[4 * h]; v[4 * h + 1] = byte_f32<1>(q[h]) * scale[4 * h + 1];
+            v[4 * h + 2] = byte_f32<2>(q[h]) * scale[4 * h + 2]; v[4 * h + 3] = byte_f32<3>(q[h]) * scale[4 * h + 3];
         } else {
             const hw_f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
             v[4 * h] = a[0] * scale[4 * h]; v[4 * h + 1] = a[1] * scale[4 * h + 1];
@@ -164,15 +173,9 @@ __device__ __forceinline__ void q8_unpack8(u32x2_t q, const float* scale, const 
         }
     }
 }
-template <int FMT>
-__device__ __forceinline__ void q8_scales(u32x2_t e, float* scale, float* s128) {
+__device__ __forceinline__ void q8_scales(u32x2_t e, float* scale) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const unsigned code = (e[j >> 2] >> (8 * (j & 3))) & 0xffu;
-        // (an infinite scale makes every int8 value NaN by itself: u * inf - inf)
-        scale[j] = FMT == HIFIC_Q_INT8 ? __uint_as_float(code << 23) : q8_scale(code);
-        s128[j] = FMT == HIFIC_Q_INT8 ? -128.f * scale[j] : 0.f;
-    }
+    for (int j = 0; j < 8; ++j) scale[j] = q8_scale((e[j >> 2] >> (8 * (j & 3))) & 0xffu);
 }
 
 // eight normalised values of a channel whose ReLU follows, as x = xh / scale, with v = fma(gamma, xh, beta) and gs = gamma * scale:

@@ -100,14 +100,14 @@ __global__ __launch_bounds__(256) void act8_restore_kernel(const u8_t* __restric
     const int c0 = (int)(rest - img * cgs) * CH;
     const unsigned hw0 = V == 1 ? oct : umin(oct * 8, (unsigned)HW - 8);
     const size_t base = ((size_t)img * C + c0) * HW + hw0;
-    float s[V], s128[V];
-    if constexpr (V == 8) q8_scales<FMT>(*(const u32x2_a1*)(qe + (size_t)img * HW + hw0), s, s128);
+    float s[V];
+    if constexpr (V == 8) q8_scales(*(const u32x2_a1*)(qe + (size_t)img * HW + hw0), s);
     else s[0] = q8_scale(qe[(size_t)img * HW + hw0]);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
         if (c0 + k >= C) break;
         float v[V];
-        if constexpr (V == 8) q8_unpack8<FMT>(*(const u32x2_a1*)(q + base + (size_t)k * HW), s, s128, v);
+        if constexpr (V == 8) q8_unpack8<FMT>(*(const u32x2_a1*)(q + base + (size_t)k * HW), s, v);
         else v[0] = q8_value<FMT>(q[base + (size_t)k * HW]) * s[0];
         if (gamma)
 #pragma unroll
@@ -160,9 +160,9 @@ __global__ __launch_bounds__(256) void act8_restore_rows_kernel(const u8_t* __re
     const long long row = i / octs;
     const unsigned c = umin((unsigned)(i - row * octs) * 8, (unsigned)C - 8);
     const unsigned e = 0x01010101u * qe[row];
-    float s[8], s128[8], v[8];
-    q8_scales<FMT>(u32x2_t{e, e}, s, s128);
-    q8_unpack8<FMT>(*(const u32x2_a1*)(q + (size_t)row * C + c), s, s128, v);
+    float s[8], v[8];
+    q8_scales(u32x2_t{e, e}, s);
+    q8_unpack8<FMT>(*(const u32x2_a1*)(q + (size_t)row * C + c), s, v);
     if (gamma)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {

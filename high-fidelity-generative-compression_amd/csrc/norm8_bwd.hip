@@ -122,13 +122,13 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_bwd_tile_kernel(const NormBw
             if constexpr (MODE == M_RMS) if (p.dstream) ds[k].load(at((const T*)p.dstream + img, oT));
         }
         V8<float> r; r.load(p.rstd + tok);
-        float sc[8], s128[8];
-        if constexpr (SRC != SRC_T) q8_scales<SRC>(*(const u32x2_a1*)(p.qe + tok), sc, s128);
+        float sc[8];
+        if constexpr (SRC != SRC_T) q8_scales(*(const u32x2_a1*)(p.qe + tok), sc);
         auto values = [&](int k, float* xh) {
             if constexpr (SRC == SRC_T) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * r.get(j);
-            } else q8_unpack8<SRC>(q[k], sc, s128, xh);
+            } else q8_unpack8<SRC>(q[k], sc, xh);
         };
         float s1[8], s2[8];
 #pragma unroll
@@ -236,13 +236,13 @@ __global__ __launch_bounds__(row_block(L)) void rms_bwd_rows_kernel(const NormBw
             if (p.dstream) ds[k].load((const T*)p.dstream + at);
         }
         const float r = p.rstd[row];
-        float sc[8], s128[8];
-        if constexpr (SRC != SRC_T) { const unsigned e = 0x01010101u * p.qe[row]; q8_scales<SRC>(u32x2_t{e, e}, sc, s128); }
+        float sc[8];
+        if constexpr (SRC != SRC_T) { const unsigned e = 0x01010101u * p.qe[row]; q8_scales(u32x2_t{e, e}, sc); }
         auto values = [&](int k, float* xh) {
             if constexpr (SRC == SRC_T) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) xh[j] = hr[k].get(j) * r;
-            } else q8_unpack8<SRC>(q[k], sc, s128, xh);
+            } else q8_unpack8<SRC>(q[k], sc, xh);
         };
         float s2 = 0.f;
 #pragma unroll

@@ -121,9 +121,9 @@ __global__ __launch_bounds__(256) void wgrad8_taps_kernel(const WgTaps p, bf16_t
                     eb[h] = __builtin_amdgcn_perm(ew[1], ew[0], sl[h]) | __builtin_amdgcn_perm(ew[3], ew[2], sh[h]);
                 }
             }
-            float sc[8], s128[8];
-            q8_scales<SRC>(eb, sc, s128);
-            q8_unpack8<SRC>(q, sc, s128, v);
+            float sc[8];
+            q8_scales(eb, sc);
+            q8_unpack8<SRC>(q, sc, v);
         } else {
             keep = 0;
 #pragma unroll

@@ -1,0 +1,83 @@
+"""The 8-bit activation operators at the ends of the value range: tokens of the largest numbers, weights and values that are not finite,
+sums of squares beyond float32.  Shapes reach every kernel: rows (one lane group, a wave, a workgroup, 1024 threads, too wide), rows of
+few channels, planes in tiles of four and eight waves, tiny planes, planes too wide for a tile."""
+import math
+
+import pytest
+import torch
+
+from oracle import act8_oracle as O
+
+pytestmark = pytest.mark.gpu
+F32 = 32 * 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+# (at least six tokens each)
+SHAPES = [(7, 5), (6, 40), (6, 41), (9, 300), (6, 960), (6, 9000), (6, 16500), (2, 40, 8, 8), (2, 21, 3, 5), (1, 700, 9, 9), (3, 20, 1, 3), (2, 4100, 2, 5)]
+
+
+def _rand(shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def _tokens(x):
+    """[tokens, C] of x [N, C, ...], and the way back."""
+    shape = x.shape
+    flat = x.movedim(1, -1).reshape(-1, shape[1]).clone()
+    return flat, lambda f: f.reshape(shape[:1] + shape[2:] + shape[1:2]).movedim(-1, 1).contiguous()
+
+
+def _with_tops(shape, dt, tops, seed=1):
+    """Token i holds tops[i] (of both signs, beside zeros and numbers of any size); the rest are ordinary."""
+    flat, back = _tokens(_rand(shape, seed))
+    for i, top in enumerate(tops):
+        flat[i] *= 0.2 * top                             # (normal numbers, clipped to the largest)
+        flat[i].clamp_(-top, top)
+        flat[i, 1], flat[i, 2], flat[i, 3], flat[i, 4] = top, 0.0, -top, -0.0
+        flat[i, 0] = 1.0 if i % 2 else -0.3 * top
+    return back(flat.to(dt))
+
+
+def _check_checkpoint(ops, x, fmt, dev):
+    a = ops.checkpoint8(x.to(dev), fmt=fmt)
+    back32, back16 = ops.restore8(a, torch.float32).cpu(), ops.restore8(a).cpu()
+    want, e = O.quantise(x.double(), fmt)
+    assert torch.equal(a.e.cpu().double() - 127, e)
+    assert torch.equal(O.values(a.q.cpu(), a.e.cpu()), want)
+    assert torch.isfinite(back32).all() and torch.equal(back32.double(), want) and torch.equal(back16.double(), want)
+    return a, want
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_tokens_of_the_top_octave_restore_to_what_was_kept(hific, dev, shape, dt, fmt):
+    """Around 127 * 2^120 (1.69e38), where a scale of 2^121 times 128 leaves float32, up to 127 * 2^121, the largest int8 value."""
+    from hific_amd import ops
+    tops = [1.6e38, 127 * 2.0 ** 120, 1.70e38, 2e38, 3e38, 127 * 2.0 ** 121 if fmt == "int8" else 448 * 2.0 ** 119]
+    _check_checkpoint(ops, _with_tops(shape, TYPES[dt], tops), fmt, dev)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("transposed,n,c,h,w,k,r,stride,reflect", [
+    (False, 2, 20, 9, 11, 24, 3, 1, False), (False, 1, 18, 21, 19, 33, 3, 2, True), (False, 2, 12, 6, 5, 9, 3, 1, False), (True, 2, 24, 9, 8, 40, 3, 2, False)])
+def test_weight_gradients_of_the_top_octave(hific, dev, transposed, n, c, h, w, k, r, stride, reflect, fmt):
+    """Exact products (of 2^121-sized values with gradients of 1e-9), at most 400 additions in a row in float32."""
+    from hific_amd import act8, lib, ops
+    pad = r // 2
+    x = _with_tops((n, c, h, w), torch.float32, [1.6e38, 1.7e38, 2e38, 3e38], seed=3)
+    a = ops.checkpoint8(x.to(dev), fmt=fmt)
+    oh, ow = ((h - 1) * stride - 2 * pad + r + stride - 1, (w - 1) * stride - 2 * pad + r + stride - 1) if transposed else (
+        (h + 2 * pad - r) // stride + 1, (w + 2 * pad - r) // stride + 1)
+    dy = _rand((n, k, oh, ow), 4, torch.bfloat16, 1e-9)
+    v = O.values(a.q.cpu(), a.e.cpu())
+    if transposed:
+        got = ops.conv_transpose2d_weight_grad8(a, dy.to(dev), (r, r), stride, pad, stride - 1)
+        ref = lambda xv, d: O.conv2d_weight_grad(torch.nn.functional.pad(d, (pad, pad + stride) * 2), xv, (r, r), stride, (0, 0, 0, 0), False)  # noqa: E731
+    else:
+        got = ops.conv2d_weight_grad8(a, dy.to(dev), (r, r), stride, (pad,) * 4, lib.PAD_REFLECT if reflect else lib.PAD_ZERO)
+        ref = lambda xv, d: O.conv2d_weight_grad(xv, d, (r, r), stride, (pad,) * 4, reflect)  # noqa: E731
+    got = got.cpu().double()
+    want, size = ref(v, dy.double()), ref(v.abs(), dy.double().abs())
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= 400 * 2.0 ** -24 * size + 1e-30).all()
