@@ -7,7 +7,8 @@
 // Powers of two, not max|v| / QMAX: q * 2^e then has at most 8 significant bits, so a restored value is EXACT in bfloat16 and a
 // product over restored values carries the one rounding of q and no second one; the price is up to one bit of int8's range
 // (e4m3 loses nothing: it has its own exponent).  qe = 255 marks a token with an infinity or NaN: it restores to NaN as a
-// whole, so that a diverged activation never comes back finite.  A token of zeros has qe = 1 (2^-126).
+// whole, so that a diverged activation never comes back finite; a finite token comes back finite (q8_top).  A token of zeros has
+// qe = 1 (2^-126).
 #pragma once
 #include "common.h"
 
@@ -36,6 +37,14 @@ __device__ __forceinline__ float q8_scale(unsigned code) {           // 2^(code 
 }
 __device__ __forceinline__ float q8_inv_scale(unsigned code) {       // 2^(127 - code); 0 for a token that is not finite
     return code == 255u ? 0.f : __uint_as_float((254u - code) << 23);
+}
+
+// v, limited to what rounds to a number of float32: at the largest exponent (2^122 for int8, 2^120 for e4m3) half way to 64 and 256 and
+// beyond, the nearest value would be 2^128, and a finite token would come back infinite.  The constants are the numbers below
+// 63.5 * 2^122 and 248 * 2^120; no token of a smaller exponent holds more than 127 * 2^121 (which still rounds to itself) or 448 * 2^119.
+template <int FMT> __device__ __forceinline__ float q8_top(float v) {
+    const float m = __uint_as_float(FMT == HIFIC_Q_INT8 ? 0x7f7dffffu : 0x7f77ffffu);
+    return __builtin_amdgcn_fmed3f(v, -m, m);
 }
 
 // One value t = v / scale -> its 8 bits (round half to even).  The clamp only acts where max|v| was formed with another rounding

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x,
         const float inv = q8_inv_scale(code);
         if (!ok) continue;               // (the last round only)
         if (g == 0) qe[tok] = (u8_t)code;
-        for (int c = g; c < C; c += G) q[base + (size_t)c * HW] = (u8_t)q8_round<FMT>(DT<T>::ld(x + base + (size_t)c * HW) * inv);
+        for (int c = g; c < C; c += G) q[base + (size_t)c * HW] = (u8_t)q8_round<FMT>(q8_top<FMT>(DT<T>::ld(x + base + (size_t)c * HW)) * inv);
     }
 }
 
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(64 * NW) void act8_pack_tile_kernel(const T* __rest
         if (c < C) {
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = xr[k].get(j) * inv[j];
+            for (int j = 0; j < 8; ++j) t[j] = q8_top<FMT>(xr[k].get(j)) * inv[j];
             *(u32x2_a1*)at(q + img, off + k * kst) = q8_pack8<FMT, false>(t);
         }
     }
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(row_block(L)) void act8_pack_rows_kernel(const T* _
         if (c < (unsigned)C) {
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = xr[k].get(j) * inv;
+            for (int j = 0; j < 8; ++j) t[j] = q8_top<FMT>(xr[k].get(j)) * inv;
             *(u32x2_a1*)(q + base + umin(c, (unsigned)C - 8)) = q8_pack8<FMT, false>(t);
         }
     }

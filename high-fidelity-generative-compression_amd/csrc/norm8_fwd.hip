@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
             float o = MODE == M_RMS ? xh * p.w[c] : fmaf(p.w[c], xh, p.b[c]);
             if (FMT != Q_NONE && ok)
                 p.q[base + c * cs] = (u8_t)(MODE == M_CHAN && p.relu ? q8_round_masked<F>(xh, inv, scale, p.w[c], p.b[c])
-                                                                     : q8_round<F>((MODE == M_RMS && p.q_of_y ? o : xh) * inv));
+                                                                     : q8_round<F>((MODE == M_RMS && p.q_of_y ? q8_top<F>(o) : xh) * inv));
             if (MODE == M_CHAN && p.relu) o = relu_nan(o);
             if (MODE == M_CHAN && rs) {      // both terms rounded to the storage type first, as norm and add one after the other
                 T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
                 float o = fmaf(p.w[c], (stream(c) - mu) * r, p.b[c]);
                 if (p.relu) o = relu_nan(o);
                 T t; DT<T>::st(&t, o); o = DT<T>::ld(&t) + DT<T>::ld(rs + c * cs);
-                if (ok) p.q2[base + c * cs] = (u8_t)q8_round<F>(o * inv2);
+                if (ok) p.q2[base + c * cs] = (u8_t)q8_round<F>(q8_top<F>(o) * inv2);
             }
         }
     }
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
         if constexpr (FMT != Q_NONE) {
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (MODE == M_RMS && p.q_of_y ? o[j] : xh[j]) * inv[j];
+            for (int j = 0; j < 8; ++j) t[j] = (MODE == M_RMS && p.q_of_y ? q8_top<F>(o[j]) : xh[j]) * inv[j];
             u32x2_t q;
             if (MODE == M_CHAN && p.relu) {
                 float gs[8];             // gamma * scale; the scale 1 / inv is a power of two (2^127 for a token that is not finite: its values are NaN)
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
             if (c >= p.C) continue;
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (xr[k].get(j) + rr[k].get(j)) * st_inv[pl * 8 + j];
+            for (int j = 0; j < 8; ++j) t[j] = q8_top<F>(xr[k].get(j) + rr[k].get(j)) * st_inv[pl * 8 + j];
             *(u32x2_a1*)at(p.q2 + img, off + k * kst) = q8_pack8<F, false>(t);
         }
     }
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
         if constexpr (FMT != Q_NONE) {
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (p.q_of_y ? o[j] : xh[j]) * inv;
+            for (int j = 0; j < 8; ++j) t[j] = (p.q_of_y ? q8_top<F>(o[j]) : xh[j]) * inv;
             *(u32x2_a1*)(p.q + at) = q8_pack8<F, true>(t);
         }
         if (p.y) { V8<T> t; t.set(o); t.store((T*)p.y + at); }

@@ -138,8 +138,8 @@ int hific_channelnorm_bwd(const void* x, const void* dy, const float* gamma, con
  * No counterpart in the reference: its training keeps every activation in float32 (autograd of src/network/generator.py:145-168).
  * A token is one position of an activation [N, C, HW] (HW = 1: rows).  q [N, C, HW] bytes: int8 (fmt 0) or e4m3 (fmt 1: finite
  * only, largest value 448); qe [N, HW] bytes: exponent + 127.  value = q * 2^(qe - 127), qe the smallest exponent with
- * max|v| <= QMAX * 2^(qe - 127) over the token's C values, QMAX = 127 or 448.  qe = 255: the token held an infinity or NaN and
- * restores to NaN.  All tensors contiguous; no alignment is needed.  Planes of eight positions and more (up to 2048 channels;
+ * max|v| <= QMAX * 2^(qe - 127) over the token's C values, QMAX = 127 or 448 (1 <= qe).  qe = 255: the token held an infinity or NaN
+ * and restores to NaN.  A finite token restores to finite values: where the nearest value would be 2^128, the one below it is kept.  All tensors contiguous; no alignment is needed.  Planes of eight positions and more (up to 2048 channels;
  * 4096 in bfloat16) and rows (HW = 1) of 8 to 16384 channels cross memory once; other shapes are read two or three times.
  * x, y, resid, dy, ... are of `dtype`; weights, statistics and their gradients float32.  At most 2^20 channels in what forms a
  * token's sums or exponent. */

@@ -45,7 +45,8 @@ def nearest(t, fmt):
 
 def quantise(v, fmt, gamma=None, beta=None):
     """(values q * 2^e, exponents [N, ...]) of float64 v.  With gamma / beta ([C]): rounded to the side of the ReLU that v is on.
-    A token with an infinity or NaN gives NaN and exponent 128."""
+    A token with an infinity or NaN gives NaN and exponent 128.  Where the nearest value would leave float32 (2^128) it is the next one
+    towards zero: a finite token stays finite."""
     v = v.double()
     bad = ~torch.isfinite(v).all(1, keepdim=True)
     vv = torch.where(bad, torch.zeros_like(v), v)
@@ -58,6 +59,8 @@ def quantise(v, fmt, gamma=None, beta=None):
         wrong = (ga * (g[idx] * torch.exp2(e)) + be > 0) != (ga * vv + be > 0)
         other = torch.where(t > g[idx], idx + 1, idx - 1).clamp(0, len(g) - 1)
         idx = torch.where(wrong, other, idx)
+    over = g[idx].abs() * torch.exp2(e) >= 2.0 ** 128
+    idx = torch.where(over, torch.where(g[idx] > 0, idx - 1, idx + 1), idx)
     out = torch.where(bad, torch.full_like(v, float("nan")), g[idx] * torch.exp2(e))
     return out, torch.where(bad, torch.full_like(e, 128.0), e).squeeze(1)
 
