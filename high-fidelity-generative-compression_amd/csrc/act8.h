@@ -18,9 +18,11 @@ typedef unsigned char u8_t;
 typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 
-// |v| as unsigned bits: ordered like the magnitudes, infinities above every number and NaN above those (fmaxf would lose a NaN)
+// |v| as unsigned bits: ordered like the magnitudes, infinities above every number and NaN above those
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+// a maximum that keeps a NaN (fmaxf drops it; one instruction either way)
+__device__ __forceinline__ float nmax(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ unsigned umin(unsigned a, unsigned b) { return a < b ? a : b; }
 
 // amax as abs_bits -> the byte of the exponent.  QMAX = 1.984375 * 2^6 (127) or 1.75 * 2^8 (448).
@@ -235,7 +237,7 @@ template <typename T> __device__ __forceinline__ const T* at(const T* base, unsi
 // (LPX < 8) is one value.  Eight values over 4 sub-groups: 12 instructions, where shuffles with selects took about 90 and the two
 // or three reductions of a tile more than the arithmetic of its values.
 template <bool MAX> __device__ __forceinline__ unsigned tile_op(unsigned x, unsigned y) { return MAX ? umax(x, y) : x + y; }
-template <bool MAX> __device__ __forceinline__ float tile_op(float x, float y) { return MAX ? fmaxf(x, y) : x + y; }
+template <bool MAX> __device__ __forceinline__ float tile_op(float x, float y) { return MAX ? nmax(x, y) : x + y; }
 template <bool MAX, typename V>
 __device__ __forceinline__ V tile_swap32(V x, V y) {
     const u32x2_t r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
@@ -332,8 +334,8 @@ template <int NW, int TP> __device__ __forceinline__ float waves_sum(const float
     return s;
 }
 template <int NW, int TP> __device__ __forceinline__ float waves_max(const float (*red)[TP], int i) {
-    float m = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
-    if constexpr (NW == 8) m = fmaxf(m, fmaxf(fmaxf(red[4][i], red[5][i]), fmaxf(red[6][i], red[7][i])));
+    float m = nmax(nmax(red[0][i], red[1][i]), nmax(red[2][i], red[3][i]));
+    if constexpr (NW == 8) m = nmax(m, nmax(nmax(red[4][i], red[5][i]), nmax(red[6][i], red[7][i])));
     return m;
 }
 

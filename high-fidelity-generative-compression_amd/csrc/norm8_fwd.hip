@@ -129,7 +129,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
             if (ok && g + G * k < p.C) xr[k].store(at((T*)p.h + img, (off + k * kst) * (unsigned)sizeof(T)));
         }
     }
-    // maxima as floats: a NaN is lost in them, but not in the sum of squares, and r carries it into the exponent
+    // maxima as floats, NaN included: r carries one of x into the exponent, but not one of a weight (or of infinity times a zero weight)
     float mu[8], acc[8], am[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) { mu[j] = 0.f; acc[j] = 0.f; am[j] = 0.f; }
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
             for (int j = 0; j < 8; ++j) {
                 const float d = xr[k].get(j) - mu[j];
                 acc[j] += d * d;
-                if (FMT != Q_NONE) am[j] = fmaxf(am[j], fabsf(MODE == M_RMS && p.q_of_y ? d * w[k] : d));
+                if (FMT != Q_NONE) am[j] = nmax(am[j], fabsf(MODE == M_RMS && p.q_of_y ? d * w[k] : d));
             }
 #pragma unroll
     for (int k = 0; k < CPT; ++k) xr[k].forget();
@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
             if constexpr (RES) {         // both terms rounded to the storage type first, as norm and add one after the other
                 V8<T> t; t.set(o);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { o[j] = t.get(j) + rr[k].get(j); if (FMT != Q_NONE) am[j] = fmaxf(am[j], fabsf(o[j])); if (o[j] != o[j]) am[j] = INFINITY; }
+                for (int j = 0; j < 8; ++j) { o[j] = t.get(j) + rr[k].get(j); if (FMT != Q_NONE) am[j] = nmax(am[j], fabsf(o[j])); }
                 xr[k] = t;               // q2 below: the sum again from its two terms, in float32
             }
         }
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
     }
     if constexpr (MODE == M_CHAN && FMT != Q_NONE && RES) {
         if (!p.q2) return;
-        tile_reduce<LPX, true>(am, redm[wave]);          // (a NaN as an infinity; redm's readers are behind a barrier)
+        tile_reduce<LPX, true>(am, redm[wave]);          // (redm's readers are behind a barrier)
         __syncthreads();
         if (tid < TP) {
             const unsigned code = q8_code<F>(abs_bits(waves_max<NW, TP>(redm, tid)));
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
         if (p.resid) rr[k].load((const T*)p.resid + base + c);
         w[k].load(p.w + c);
     }
-    float ss = 0.f, am = 0.f;            // (a NaN is lost in am, not in ss, and r carries it into the exponent)
+    float ss = 0.f, am = 0.f;            // (am keeps a NaN: it may be a weight's)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const unsigned cn = (unsigned)(l + L * k) * 8, c = umin(cn, C - 8);
@@ -272,14 +272,14 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
             // a group past the end was moved back: its first values belong to the group before it
             const float v = c + j >= cn ? xr[k].get(j) : 0.f;
             ss += v * v;
-            if (FMT != Q_NONE) am = fmaxf(am, fabsf(p.q_of_y ? v * w[k].get(j) : v));
+            if (FMT != Q_NONE) am = nmax(am, fabsf(p.q_of_y ? v * w[k].get(j) : v));
         }
     }
     ss = row_sum<L>(ss);
     const float r = rsqrtf(ss * p.rv + p.eps);
     float inv = 0.f;
     if constexpr (FMT != Q_NONE) {
-        const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(__float_as_uint(am))) * r));
+        const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(abs_bits(am))) * r));
         inv = q8_inv_scale(code);
         if (ok && l == 0) p.qe[row0] = (u8_t)code;
     }

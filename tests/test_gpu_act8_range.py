@@ -100,3 +100,36 @@ def test_finite_tokens_stay_finite_up_to_the_types_maximum(hific, dev, shape, dt
         want, e = O.quantise(rs.double(), fmt)
         assert torch.equal(a.e.cpu().double() - 127, e)
         assert torch.equal(torch.nan_to_num(ops.restore8(a, torch.float32).cpu().double()), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rms_norm8_of_weights_and_values_that_are_not_finite(hific, dev, shape, dt, fmt):
+    """A token whose output holds an infinity or NaN is not finite as a whole, wherever that came from: a NaN or an infinity among the
+    weights (times a zero too), or an infinite value in a channel of weight zero.  The other tokens are as without it."""
+    from hific_amd import ops
+    t = TYPES[dt]
+    x, w = _rand(shape, 11, t), 1.0 + 0.3 * _rand((shape[1],), 12)
+    w[1] = 0.0
+
+    def run(xv, wv):
+        a = ops.rms_norm8(xv.to(dev), wv.to(dev), fmt=fmt)
+        return a.e.cpu(), ops.restore8(a, torch.float32).cpu()
+    e0, good = run(x, w)
+    assert torch.isfinite(good).all() and not (e0 == 255).any()
+    flat, back = _tokens(x)
+    flat[0, 3] = 0.0
+    for value in (float("nan"), float("inf"), float("-inf")):
+        bad = w.clone()
+        bad[3] = value
+        e, got = run(back(flat), bad)
+        assert (e == 255).all() and torch.isnan(got).all(), value
+    flat[0, 3] = x.movedim(1, -1).reshape(-1, shape[1])[0, 3]
+    flat[2, 1] = float("inf")                            # (its weight is zero)
+    flat[4, 0], flat[5, 4] = float("-inf"), float("nan")
+    e, got = run(back(flat), w)
+    hit = ~torch.isfinite(back(flat)).all(1)
+    assert hit.sum() == 3 and torch.equal(e == 255, hit)
+    hit = hit.unsqueeze(1).expand(shape)
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], good[~hit])
