@@ -486,10 +486,10 @@ def _weight_grad(kept, relu, dz, dw, acc, geom, cd):
         lib.call("hific_conv2d_bwd_weight", ptr(x), ptr(dz), ptr(dw), N, C, H, W, K, R, S, *geom, acc, cd, flags, *ops._ws(x), stream())
 
 
-def _conv_backward(ctx, kept, relu, dz, weight, want_x, want_w, after=None):
-    """Data gradient on the current stream; weight gradient (and `after`) next to it on the side stream where the parameters live in
-    an arena, as ops.ConvNormFn does.  -> dx, dw"""
-    side = want_w and ops._use_side(ctx.w_slot)
+def _conv_backward(ctx, kept, relu, dz, weight, want_x, want_w, after=None, after_slot=None):
+    """Data gradient on the current stream; weight gradient (and `after`, which writes `after_slot`) next to it on the side stream where
+    every gradient made there is written into an arena: one that autograd gets is read on the current stream at once.  -> dx, dw"""
+    side = want_w and ops._use_side(ctx.w_slot, after_slot if after is not None else True)
     ev = lib.stream_obj().record_event() if side else None
     dx = _conv_bwd_data(dz, weight, ctx.geom, ctx.x_shape, ctx.x_dtype, ctx.mode) if want_x else None
     dw = None
@@ -612,7 +612,7 @@ class Conv8Fn(Function):
             dbt, acc, db = ops._grad_target(ctx.b_slot, weight.new_empty(K))
             lib.call("hific_channel_sum", ptr(dy), ptr(dbt), dy.shape[0], K, plane, acc, lib.dtype_code(dy), *ops._ws(dy), stream())
         with _on(dy):
-            dx, dw = _conv_backward(ctx, (q, e, xg, xb), ctx.xrelu, dy, weight, need[0], need[6], bias if want_b else None)
+            dx, dw = _conv_backward(ctx, (q, e, xg, xb), ctx.xrelu, dy, weight, need[0], need[6], bias if want_b else None, ctx.b_slot)
             if want_b:
                 ops._written(ctx.b_slot)
         return (dx, None, None, None, None, None, dw, db, None, None, None)

@@ -1,0 +1,47 @@
+"""conv2d(x8=) with its parameters in and out of an arena, the side stream on and off, and an input whose gamma / beta nothing else
+holds: the same gradients."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(shape, seed, dtype=torch.float32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+@pytest.fixture(autouse=True)
+def _mode(hific):
+    from hific_amd import ops
+    was = ops.get_compute_dtype(), ops._SIDE_ON
+    hific.set_compute_dtype(torch.bfloat16)
+    yield
+    hific.set_compute_dtype(was[0])
+    ops.set_side_stream(was[1])
+
+
+@pytest.mark.parametrize("in_arena", ["none", "weight", "bias", "both"])
+def test_conv_with_an_8_bit_input_and_part_of_its_parameters_in_an_arena(hific, dev, in_arena):
+    from hific_amd import ops, optim
+    x, dy = _rand((4, 48, 40, 40), 1, torch.bfloat16).to(dev), _rand((4, 64, 40, 40), 2, torch.bfloat16).to(dev)
+    a = ops.checkpoint8(x)
+    res = []
+    for side in (False, True):
+        ops.set_side_stream(side)
+        w = torch.nn.Parameter(_rand((64, 48, 3, 3), 3).to(dev))
+        b = torch.nn.Parameter(_rand((64,), 4).to(dev))
+        members = [p for p, n in ((w, "weight"), (b, "bias")) if in_arena in (n, "both")]
+        arena = optim.ParamArena(members) if members else None
+        for rep in range(3):                             # (the later passes add)
+            xd = x.clone().requires_grad_()
+            y = ops.conv2d(xd, w, b, 1, (1, 1, 1, 1), x8=a)
+            # the bias gradient is read as soon as autograd has it
+            y.backward(dy)
+        torch.cuda.synchronize()
+        res.append((w.grad.clone(), b.grad.clone(), xd.grad.clone()))
+        assert arena is None or len(arena.slots) == len(members)
+    for p, q in zip(*res):
+        assert torch.equal(p, q)
+    want = 3 * dy.double().sum((0, 2, 3))
+    assert ((res[1][1].double() - want).abs() <= 3 * 6400 * 2.0 ** -24 * dy.double().abs().sum((0, 2, 3))).all()
