@@ -502,7 +502,7 @@ def _conv_backward(ctx, kept, relu, dz, weight, want_x, want_w, after=None, afte
         if after is not None:
             after()
     if side:
-        with ops._SideLaunch(ev, kept[0], kept[1], dz, key=ctx.w_slot):
+        with ops._SideLaunch(ev, *kept, dz, key=ctx.w_slot):
             params()
     else:
         params()

@@ -75,3 +75,23 @@ def test_gradients_handed_to_autograd_come_from_the_main_stream(launches, w_in, 
         assert by["hific_channel_sum"][0] == "main" and by["hific_channel_sum"][1][1] == db.data_ptr()
     if w_in and b_in:
         assert by["weight"][0] == by["hific_channel_sum"][0] == "side"
+
+
+@pytest.mark.parametrize("arena", [False, True])
+def test_the_side_stream_holds_everything_that_its_launches_read(launches, arena):
+    """gamma and beta of an Act8 may be temporaries (a computed gamma) that the node alone holds: their memory must not go back to the
+    allocator before the side stream has read them."""
+    weight, bias = torch.zeros(6, 4, 3, 3), torch.zeros(6)
+    q, e = torch.zeros(2, 4, 5, 5, dtype=torch.int8), torch.full((2, 5, 5), 127, dtype=torch.uint8)
+    gamma, beta = torch.ones(4), torch.zeros(4)
+    ctx = _ctx(weight, bias, _Slot(weight) if arena else None, _Slot(bias) if arena else None, q, e, gamma, beta)
+    dy = torch.zeros(2, 6, 5, 5, dtype=torch.bfloat16)
+    with torch.no_grad():
+        act8.Conv8Fn.backward(ctx, dy)
+    read = [args[:4] for name, stream, args in launches.calls if name == "weight" and stream == "side"]
+    assert bool(read) == arena
+    held = {t.data_ptr() for t in launches.kept}
+    for ptrs in read:
+        assert set(ptrs) <= held, "an operand of a side-stream launch is not recorded there"
+    if arena:
+        assert dy.data_ptr() in held

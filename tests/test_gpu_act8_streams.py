@@ -45,3 +45,30 @@ def test_conv_with_an_8_bit_input_and_part_of_its_parameters_in_an_arena(hific, 
         assert torch.equal(p, q)
     want = 3 * dy.double().sum((0, 2, 3))
     assert ((res[1][1].double() - want).abs() <= 3 * 6400 * 2.0 ** -24 * dy.double().abs().sum((0, 2, 3))).all()
+
+
+def test_an_input_whose_norm_parameters_are_temporaries(hific, dev):
+    """gamma = 1 + p is held by the node alone; once the node is done its memory is the main stream's to use again."""
+    from hific_amd import ops, optim
+    C = 48
+    x, dy = _rand((4, C, 40, 40), 11, torch.bfloat16).to(dev), _rand((4, 64, 40, 40), 12, torch.bfloat16).to(dev)
+    p, beta = (0.2 * _rand((C,), 13)).to(dev), (0.2 * _rand((C,), 14)).to(dev)
+    kept = ops.checkpoint8(x)
+    res = []
+    for side in (False, True):
+        ops.set_side_stream(side)
+        w, b = (torch.nn.Parameter(_rand(s, n).to(dev)) for s, n in (((64, C, 3, 3), 15), ((64,), 16)))
+        optim.ParamArena([w, b])
+        for rep in range(3):
+            a = ops.Act8(kept.q, kept.e, 1 + p, beta + 0, True)
+            y = ops.conv2d(ops.restore8(a), w, b, 1, (1, 1, 1, 1), x8=a)
+            del a
+            y.backward(dy)
+            del y
+            for _ in range(8):
+                torch.full((C,), float("nan"), device=dev)
+        torch.cuda.synchronize()
+        res.append((w.grad.clone(), b.grad.clone()))
+    assert torch.isfinite(res[0][0]).all()
+    for s, t in zip(*res):
+        assert torch.equal(s, t)
