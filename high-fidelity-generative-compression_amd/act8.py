@@ -101,10 +101,40 @@ def _on(t):
     return _here if t.get_device() == lib._cur_device() else torch.cuda.device(t.device)
 
 
-def _first_order(*grads):
-    # grad mode is on in a backward pass with create_graph=True only
-    if torch.is_grad_enabled() and any(g is not None and g.requires_grad for g in grads):
-        raise lib.HificError("the 8-bit activation operators have no second derivative")
+class _SecondOrder(Function):
+    """Passes gradients on; differentiating them raises."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise lib.HificError(_NO_SECOND)
+
+
+_NO_SECOND = "the 8-bit activation operators have no second derivative"
+
+
+def _first_order(backward):
+    """A backward pass that has no derivative of its own.  Grad mode is on in it with create_graph=True only: an incoming gradient that
+    requires grad is refused, and what is computed from the saved tensors raises where it is differentiated in turn - returned as
+    constants, a penalty on it would drop out of another loss without a word.  Gradients that are passed through are constants in truth."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        if any(g is not None and g.requires_grad for g in grads):
+            raise lib.HificError(_NO_SECOND)
+        with torch.no_grad():
+            grads = [g if g is None else c16(g) for g in grads]
+            out = backward(ctx, *grads)
+        made = {id(g): g for g in out if g is not None and not any(g is t for t in grads)}
+        if not made:
+            return out
+        made = dict(zip(made, _SecondOrder.apply(*(g.detach().requires_grad_() for g in made.values()))))
+        return tuple(made.get(id(g), g) if g is not None else None for g in out)
+    return run
 
 
 class Act8:
@@ -227,8 +257,8 @@ class RmsNormFn(Function):
         return y if h is None else (y, h)
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, dstream=None):
-        _first_order(dy, dstream)
         kept, e, rstd, weight = ctx.saved_tensors
         none = (None,) * 5
         if dy is None:                                   # only the stream was used
@@ -335,8 +365,8 @@ class ChannelNorm8Fn(Function):
         return (y,) + kept
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, _q, _e):
-        _first_order(dy)
         if dy is None:
             return (None,) * 10
         q, e, rstd, gamma, beta = ctx.saved_tensors
@@ -535,8 +565,8 @@ class ConvNorm8Fn(Function):
         return (y,) + kept
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy, _q, _e):
-        _first_order(dy)
         if dy is None:
             return (None,) * 16
         x, e, xg, xb, weight, nq, ne, rstd, gamma, beta = ctx.saved_tensors
@@ -598,8 +628,8 @@ class Conv8Fn(Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, dy):
-        _first_order(dy)
         q, e, xg, xb, weight = ctx.saved_tensors
         dy = c16(dy)
         need = ctx.needs_input_grad
