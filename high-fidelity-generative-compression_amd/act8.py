@@ -11,7 +11,7 @@ import functools
 import os
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import lib, ops
 from .lib import ptr, stream, require_gpu
@@ -294,6 +294,8 @@ def _rms_args(x, weight, resid):
 
 
 def _needs_grad(x, weight, resid):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, weight, resid)):
+        raise lib.HificError("the root-mean-square norm has no forward-mode derivative")
     return torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (resid is not None and resid.requires_grad))
 
 

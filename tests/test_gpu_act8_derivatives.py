@@ -71,3 +71,29 @@ def test_gradients_that_are_passed_through_stay_constants(hific, dev):
     y, _ = ops.channel_norm8(z, w, w, resid=rs)
     g, = torch.autograd.grad(y.sum(), rs, create_graph=True)
     assert torch.equal(g, torch.ones_like(g)) and not g.requires_grad
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "resid"])
+def test_forward_mode_is_refused(hific, dev, which):
+    """A tangent is refused, whether or not anything requires grad; without one a dual level changes nothing."""
+    import torch.autograd.forward_ad as fwd
+    from hific_amd import ops
+    t = {"x": _rand((2, 8, 6, 6), 21).to(dev), "weight": _rand((8,), 22).to(dev), "resid": _rand((2, 8, 6, 6), 23).to(dev)}
+    calls = [lambda a: ops.rms_norm(a["x"], a["weight"], resid=a["resid"]), lambda a: ops.rms_norm(a["x"], a["weight"], resid=a["resid"], fmt="int8"),
+             lambda a: ops.rms_norm8(a["x"], a["weight"], resid=a["resid"]),
+             lambda a: ops.channel_norm8(a["x"], a["weight"], t["weight"], resid=a["resid"])]
+    want = ops.rms_norm(t["x"], t["weight"], resid=t["resid"])
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), fwd.dual_level():
+            dual = dict(t, **{which: fwd.make_dual(t[which], torch.ones_like(t[which]))})
+            for i, f in enumerate(calls):
+                with pytest.raises(RuntimeError):
+                    f(dual)
+                    pytest.fail(f"call {i} lost a tangent")
+            got = ops.rms_norm(t["x"], t["weight"], resid=t["resid"])
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            x = t["x"].clone()
+            conv = lambda v: ops.conv2d(v, torch.ones(4, 8, 3, 3, device=dev), None, x8=ops.checkpoint8(x))  # noqa: E731
+            with pytest.raises(RuntimeError):
+                conv(fwd.make_dual(x, torch.ones_like(x)))
+                pytest.fail("conv2d(x8=) lost a tangent")
