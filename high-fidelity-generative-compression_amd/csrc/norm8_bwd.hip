@@ -7,7 +7,7 @@ struct NormBwd {
     void* dx; float* part;
     int C, HW; unsigned tiles; int relu, db;
     long long tokens; int nsplit;        // (tokens: tiles of the batch in norm8_bwd_tile_kernel)
-    float rc, rv;                        // as in NormFwd
+    float nc, nv;                        // as in NormFwd
 };
 
 template <typename T, int SRC>
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(256) void norm8_bwd_kernel(const NormBwd p) {
             d *= p.w[c];
             s1 += d; s2 += d * xh;
         }
-        if (MODE == M_CHAN) s1 = tok_sum<PX>(s1, red) * p.rc;
-        s2 = tok_sum<PX>(s2, red) * p.rv;
+        if (MODE == M_CHAN) s1 = tok_sum<PX>(s1, red) / p.nc;
+        s2 = tok_sum<PX>(s2, red) / p.nv;
         if (!ok) continue;               // (the last round only)
         for (int c = g; c < p.C; c += G) {
             const float xh = norm8_xh<T, SRC>(p, base + c * cs, r, scale);
@@ -161,8 +161,8 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_bwd_tile_kernel(const NormBw
         if (MODE == M_CHAN) tile_reduce<LPX, false>(s1, red[0][wave]);
         __syncthreads();
         if (tid < TP) {
-            st[1][tid] = waves_sum<NW, TP>(red[1], tid) * p.rv;
-            if (MODE == M_CHAN) st[0][tid] = waves_sum<NW, TP>(red[0], tid) * p.rc;
+            st[1][tid] = waves_sum<NW, TP>(red[1], tid) / p.nv;
+            if (MODE == M_CHAN) st[0][tid] = waves_sum<NW, TP>(red[0], tid) / p.nc;
         }
         __syncthreads();
 #pragma unroll
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(row_block(L)) void rms_bwd_rows_kernel(const NormBw
         if constexpr (K > 1)             // (unpacked again below, as in norm8_bwd_tile_kernel)
 #pragma unroll
             for (int k = 0; k < K; ++k) { dy[k].forget(); if constexpr (SRC == SRC_T) hr[k].forget(); else forget(q[k]); }
-        s2 = row_sum<L>(s2) * p.rv;
+        s2 = row_sum<L>(s2) / p.nv;
         if (!ok) continue;               // (only the last round has rows that are not there, and none of its lanes waits again)
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -369,8 +369,8 @@ size_t norm8_rows(int mode, int N, int C, int HW) {
 
 template <typename T, int MODE, int SRC>
 int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc, int acc2, size_t ws_bytes, hipStream_t st) {
-    p.rc = 1.f / (float)p.C;
-    p.rv = 1.f / (float)(MODE == M_RMS ? p.C : p.C - 1);
+    p.nc = (float)p.C;
+    p.nv = (float)(MODE == M_RMS ? p.C : p.C - 1);
     const int nr = MODE == M_RMS ? 1 : 2 + p.db;
     const size_t rows = norm8_rows<T>(MODE, N, p.C, p.HW);
     if (rows * nr * p.C * sizeof(float) > ws_bytes) return HIFIC_ERR_WS;

@@ -6,7 +6,7 @@ struct NormFwd {
     void* y; void* h; float* rstd;
     u8_t *q, *qe, *q2, *qe2;             // xh (RMS with q_of_y: y) and, with a channel norm's resid, y
     int C, HW; unsigned tiles; float eps; int relu, q_of_y;
-    float rc, rv;                        // 1 / C, and 1 / C or 1 / (C - 1): a product in the place of a division per position
+    float nc, nv;                        // C, and C or C - 1: divisors (a product with a rounded 1 / C would miss the mean of equal terms)
 };
 
 // Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2; 2x3000x32x32 250 us, which
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
         if (MODE == M_CHAN) {
             float s = 0.f;
             for (int c = g; c < p.C; c += G) s += stream(c);
-            mu = tok_sum<PX>(s, red) * p.rc;
+            mu = tok_sum<PX>(s, red) / p.nc;
         }
         float ss = 0.f;
         for (int c = g; c < p.C; c += G) {
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
             if (MODE == M_RMS && h && ok) DT<T>::st(h + c * cs, v);
         }
         ss = tok_sum<PX>(ss, red);
-        const float r = rsqrtf(ss * p.rv + p.eps);
+        const float r = rsqrtf(ss / p.nv + p.eps);
         if (p.rstd && ok && g == 0) p.rstd[tok] = r;
         unsigned code = 0;
         float inv = 0.f, scale = 0.f;
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
                 for (int j = 0; j < 8; ++j) acc[j] += xr[k].get(j);
         tile_reduce<LPX, false>(acc, red[wave]);
         __syncthreads();
-        if (tid < TP) st_r[tid] = waves_sum<NW, TP>(red, tid) * p.rc;
+        if (tid < TP) st_r[tid] = waves_sum<NW, TP>(red, tid) / p.nc;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; ++j) { mu[j] = st_r[pl * 8 + j]; acc[j] = 0.f; }
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
     __syncthreads();
     if (tid < TP) {
         const float ss = waves_sum<NW, TP>(red, tid);
-        const float r = rsqrtf(ss * p.rv + p.eps);
+        const float r = rsqrtf(ss / p.nv + p.eps);
         st_r[tid] = r;
         if (p.rstd && sok) p.rstd[stok] = r;
         if (FMT != Q_NONE) {
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
         }
     }
     ss = row_sum<L>(ss);
-    const float r = rsqrtf(ss * p.rv + p.eps);
+    const float r = rsqrtf(ss / p.nv + p.eps);
     float inv = 0.f;
     if constexpr (FMT != Q_NONE) {
         const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(abs_bits(am))) * r));
@@ -314,8 +314,8 @@ NormFwd norm8_part(NormFwd p, long long n0) {                        // from ima
 }
 template <typename T, int MODE, int FMT>
 int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
-    p.rc = 1.f / (float)p.C;
-    p.rv = 1.f / (float)(MODE == M_RMS ? p.C : p.C - 1);
+    p.nc = (float)p.C;
+    p.nv = (float)(MODE == M_RMS ? p.C : p.C - 1);
     if (p.HW >= 8) {
         const TileCfg t = tile_pick(N, p.C, p.HW, tile_most<T>(), sizeof(T));
         if (t.lpx) {

@@ -133,3 +133,31 @@ def test_rms_norm8_of_weights_and_values_that_are_not_finite(hific, dev, shape, 
     assert hit.sum() == 3 and torch.equal(e == 255, hit)
     hit = hit.unsqueeze(1).expand(shape)
     assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], good[~hit])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [5, 41, 47, 55, 61, 82, 97, 220, 301, 947, 960, 2090, 4100, 16500])
+@pytest.mark.parametrize("positions", [(), (8, 9), (1, 3)])
+def test_means_of_equal_terms_are_exact(hific, dev, channels, positions, dt):
+    """Sums of C equal terms that float32 holds exactly, divided by C, are those terms (a product with a rounded 1 / C misses them for
+    C = 41, 47, 55, ...): tokens of +-1 have the mean square 1, and a flat token of 1.5 is its own mean - normalised to zero, not to
+    roundings times rsqrt(eps)."""
+    from hific_amd import ops
+    t = TYPES[dt]
+    shape = (3, channels) + positions
+    sign = torch.where(_rand(shape, 61) > 0, 1.0, -1.0).to(t)
+    w, b = torch.ones(channels), 0.25 * _rand((channels,), 62)
+    y = ops.rms_norm(sign.to(dev), w.to(dev), eps=1e-12)
+    assert torch.equal(y.cpu(), sign)
+    # dx = r (g - xh mean(g xh)) with g = xh: nothing is left
+    x = sign.to(dev).requires_grad_()
+    dx, = torch.autograd.grad(ops.rms_norm(x, w.to(dev), eps=1e-12), x, sign.to(dev))
+    assert torch.equal(dx.cpu(), torch.zeros(shape, dtype=t))
+    flat = torch.full(shape, 1.5, dtype=t).to(dev).requires_grad_()
+    y, a = ops.channel_norm8(flat, w.to(dev), b.to(dev))
+    assert torch.equal(y.detach().cpu(), b.reshape((1, -1) + (1,) * len(positions)).expand(shape).to(t))
+    q, e, rstd, _, _ = y.grad_fn.saved_tensors
+    assert (e == 1).all() and not q.any()
+    # dx = r (g - mean(g)) with xh = 0 and equal g
+    dx, = torch.autograd.grad(y, flat, torch.full(shape, 0.75, dtype=t).to(dev))
+    assert torch.equal(dx.cpu(), torch.zeros(shape, dtype=t))
