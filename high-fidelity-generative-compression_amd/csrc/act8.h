@@ -49,6 +49,11 @@ template <int FMT> __device__ __forceinline__ float q8_top(float v) {
     return __builtin_amdgcn_fmed3f(v, -m, m);
 }
 
+// the same as a limit of t = v / scale for a token of exponent byte `code`: 63 and 240 at the largest exponent
+template <int FMT> __device__ __forceinline__ float q8_limit(unsigned code) {
+    return FMT == HIFIC_Q_INT8 ? (code == 249u ? 63.f : 127.f) : (code == 247u ? 240.f : 448.f);
+}
+
 // One value t = v / scale -> its 8 bits (round half to even).  The clamp only acts where max|v| was formed with another rounding
 // than v itself (|t| at most one ulp above QMAX).  0 * inf of a token that is not finite is stored as 0.
 template <int FMT>

@@ -277,10 +277,11 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
     }
     ss = row_sum<L>(ss);
     const float r = rsqrtf(ss / p.nv + p.eps);
-    float inv = 0.f;
+    float inv = 0.f, lim = 0.f;
     if constexpr (FMT != Q_NONE) {
         const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(abs_bits(am))) * r));
         inv = q8_inv_scale(code);
+        lim = q8_limit<F>(code);
         if (ok && l == 0) p.qe[row0] = (u8_t)code;
     }
     if (!ok) return;
@@ -296,8 +297,8 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
         if constexpr (FMT != Q_NONE) {
             float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = (p.q_of_y ? q8_top<F>(o[j]) : xh[j]) * inv;
-            *(u32x2_a1*)(p.q + at) = q8_pack8<F, true>(t);
+            for (int j = 0; j < 8; ++j) t[j] = __builtin_amdgcn_fmed3f((p.q_of_y ? o[j] : xh[j]) * inv, -lim, lim);
+            *(u32x2_a1*)(p.q + at) = q8_pack8<F, false>(t);
         }
         if (p.y) { V8<T> t; t.set(o); t.store((T*)p.y + at); }
     }
