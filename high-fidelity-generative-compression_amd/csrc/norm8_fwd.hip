@@ -9,6 +9,20 @@ struct NormFwd {
     float nc, nv;                        // C, and C or C - 1: divisors (a product with a rounded 1 / C would miss the mean of equal terms)
 };
 
+// r of a token whose sum of squares left float32 (values above about 1e19), d(c) its values: the sum again in 64 bits.  One lane walks
+// the channels: such tokens are rare, and the kernels keep no register for them.  0 where a value is infinite: it becomes NaN
+// (infinity * 0) and the others 0, as in the formula.
+template <typename D>
+__device__ float norm8_r_far(D d, int C, float nv, float eps) {
+    double ss = 0.;
+#pragma unroll 1
+    for (int c = 0; c < C; ++c) { const double v = d(c); ss += v * v; }
+    return (float)(1. / sqrt(ss / nv + eps));
+}
+__device__ __forceinline__ float norm8_r(float ss, float nv, float eps) { return rsqrtf(ss / nv + eps); }
+// max|d w| r does not give the exponent of y = (d r) w where d * w left the range of float32 or lost its bits below it
+__device__ __forceinline__ bool norm8_far(float m, float ss) { return m == INFINITY || (m < 0x1p-100f && ss > 0.f); }
+
 // Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2; 2x3000x32x32 250 us, which
 // the tiles below take in 17).
 template <typename T, int MODE, int FMT, int PX>
@@ -44,7 +58,8 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
             if (MODE == M_RMS && h && ok) DT<T>::st(h + c * cs, v);
         }
         ss = tok_sum<PX>(ss, red);
-        const float r = rsqrtf(ss / p.nv + p.eps);
+        float r = norm8_r(ss, p.nv, p.eps);
+        if (ss == INFINITY) r = norm8_r_far([&](int c) { return stream(c) - mu; }, p.C, p.nv, p.eps);
         if (p.rstd && ok && g == 0) p.rstd[tok] = r;
         unsigned code = 0;
         float inv = 0.f, scale = 0.f;
@@ -165,16 +180,31 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
     __syncthreads();
     if (tid < TP) {
         const float ss = waves_sum<NW, TP>(red, tid);
-        const float r = rsqrtf(ss / p.nv + p.eps);
-        st_r[tid] = r;
-        if (p.rstd && sok) p.rstd[stok] = r;
+        const unsigned at0 = umin(so * 8, (unsigned)p.HW - 8) + (tid & 7);       // (of the last tile's lanes past the plane: some position of it)
+        auto dev = [&](int c) {
+            const size_t i = at0 + (size_t)c * p.HW;
+            float v = DT<T>::ld(x + i);
+            if (MODE == M_CHAN) return v - st_r[tid];
+            if (RES) { T o; DT<T>::st(&o, v + DT<T>::ld(rs + i)); v = DT<T>::ld(&o); }
+            return v;
+        };
+        float r = norm8_r(ss, p.nv, p.eps);
+        if (ss == INFINITY) r = norm8_r_far(dev, p.C, p.nv, p.eps);
         if (FMT != Q_NONE) {
             // max|d| r = max|d r|: a rounded product is monotone (with q_of_y the weight comes between, and q8_pack8 clamps)
             const float m = waves_max<NW, TP>(redm, tid);
-            const unsigned code = q8_code<F>(abs_bits(m * r));
+            float top = m * r;
+            if (MODE == M_RMS && p.q_of_y && norm8_far(m, ss)) {
+                top = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < p.C; ++c) top = nmax(top, fabsf(dev(c) * r * p.w[c]));
+            }
+            const unsigned code = q8_code<F>(abs_bits(top));
             st_inv[tid] = q8_inv_scale(code);
             if (sok) p.qe[stok] = (u8_t)code;
         }
+        st_r[tid] = r;
+        if (p.rstd && sok) p.rstd[stok] = r;
     }
     __syncthreads();
     // (xh / scale in two products: r / scale overflows where a token's values are all alike or nearly so)
@@ -275,11 +305,42 @@ __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFw
             if (FMT != Q_NONE) am = nmax(am, fabsf(p.q_of_y ? v * w[k].get(j) : v));
         }
     }
+    // the widest rows unpack again below: kept unpacked, their values would cost a workgroup per CU (2048x16384 to 8 bits 28 us, 35)
+    if constexpr (sizeof(T) == 2 && (L == 1024 || K == 4))
+#pragma unroll
+        for (int k = 0; k < K; ++k) xr[k].forget();
     ss = row_sum<L>(ss);
-    const float r = rsqrtf(ss / p.nv + p.eps);
-    float inv = 0.f, lim = 0.f;
+    float r = norm8_r(ss, p.nv, p.eps), m = 0.f, inv = 0.f, lim = 0.f;
+    if (FMT != Q_NONE) m = __uint_as_float(row_max<L>(abs_bits(am)));
+    float top = m * r;
+    const bool far = ss == INFINITY || (FMT != Q_NONE && p.q_of_y && norm8_far(m, ss));
+    if (__any(far)) {                    // (from memory again: such rows are rare, and the kernel keeps no register for them)
+        auto value = [&](unsigned c) {
+            float v = DT<T>::ld((const T*)p.x + base + c);
+            if (p.resid) { T o; DT<T>::st(&o, v + DT<T>::ld((const T*)p.resid + base + c)); v = DT<T>::ld(&o); }
+            return v;
+        };
+        // norm8_r_far by all lanes of the row: in float32, scaled by the power of two that takes the largest value to [2, 4)
+        unsigned am = 0;
+#pragma unroll 1
+        for (unsigned c = l; c < C; c += L) am = umax(am, abs_bits(value(c)));
+        am = row_max<L>(am);
+        const float s = __uint_as_float(am >= 0x7f800000u ? 0u : (255u - (am >> 23)) << 23);
+        float sum = 0.f;
+#pragma unroll 1
+        for (unsigned c = l; c < C; c += L) { const float v = value(c) * s; sum += v * v; }
+        sum = row_sum<L>(sum);
+        if (ss == INFINITY) r = am >= 0x7f800000u ? 0.f : s * rsqrtf(sum / p.nv + p.eps * s * s);
+        if (FMT != Q_NONE) {
+            float y = 0.f;
+#pragma unroll 1
+            for (unsigned c = l; c < C; c += L) y = nmax(y, fabsf(p.q_of_y ? value(c) * r * p.w[c] : value(c) * r));
+            y = __uint_as_float(row_max<L>(abs_bits(y)));
+            if (far) top = y;            // (a row's result does not depend on its neighbours)
+        }
+    }
     if constexpr (FMT != Q_NONE) {
-        const unsigned code = q8_code<F>(abs_bits(__uint_as_float(row_max<L>(abs_bits(am))) * r));
+        const unsigned code = q8_code<F>(abs_bits(top));
         inv = q8_inv_scale(code);
         lim = q8_limit<F>(code);
         if (ok && l == 0) p.qe[row0] = (u8_t)code;

@@ -161,3 +161,79 @@ def test_means_of_equal_terms_are_exact(hific, dev, channels, positions, dt):
     # dx = r (g - mean(g)) with xh = 0 and equal g
     dx, = torch.autograd.grad(y, flat, torch.full(shape, 0.75, dtype=t).to(dev))
     assert torch.equal(dx.cpu(), torch.zeros(shape, dtype=t))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_norms_of_values_whose_squares_leave_float32(hific, dev, shape, dt):
+    """Values of 1e19 to the type's maximum: normalised values are of order one, as for any other size.  rstd may be as small as 2^-128,
+    where float32 has 21 bits: F32 counts 2^-19."""
+    from hific_amd import ops
+    t = TYPES[dt]
+    C = shape[1]
+    w, b = 1.0 + 0.3 * _rand((C,), 21), 0.2 * _rand((C,), 22)
+    flat, back = _tokens(_rand(shape, 23))
+    for i, size in enumerate((1e19, 3e20, 1e25, 1e33, 2e37)):
+        flat[i] *= size
+    flat[5] = torch.finfo(t).min                         # (a mask's value in every channel)
+    x = back(flat.to(t))
+    dy, rs = _rand(shape, 24, t), _rand(shape, 25, t)
+    half = torch.finfo(t).eps / 2
+    y, h, r = O.rms_norm(x, w, rs)
+    assert torch.isfinite(h).all()
+    for fmt in (None, "int8", "e4m3"):
+        leaves = [v.to(dev).requires_grad_() for v in (x, w, rs)]
+        gy, gh = ops.rms_norm(leaves[0], leaves[1], resid=leaves[2], fmt=fmt)
+        rstd = gy.grad_fn.saved_tensors[2].detach().cpu().double()
+        dx, dw = torch.autograd.grad(gy, leaves[:2], dy.to(dev))
+        assert torch.equal(gh.cpu(), h)
+        assert ((gy.cpu().double() - y).abs() <= (half + F32) * y.abs()).all(), fmt
+        assert ((rstd.unsqueeze(1) - r).abs() <= F32 * r).all()
+        assert torch.isfinite(dx).all() and torch.isfinite(dw).all()
+        xh = h.double() * r
+        if fmt is None:
+            _, wdw = O.rms_norm_grad(xh, r, w, dy)
+            terms = (dy.double() * xh).abs().sum([0] + list(range(2, x.dim())))
+            assert ((dw.cpu().double() - wdw).abs() <= 8 * F32 * terms).all()
+    a, _ = ops.rms_norm8(x.to(dev), w.to(dev), resid=rs.to(dev), fmt="int8")
+    step = torch.exp2(a.e.cpu().double() - 127).unsqueeze(1)
+    assert ((ops.restore8(a, torch.float32).cpu().double() - y).abs() <= 0.5 * step * (1 + 1e-6) + F32 * y.abs()).all()
+    # the channel norm: sums of C values have to stay in float32 (a token whose sum does not is NaN, not a quiet zero)
+    flat[4], flat[5] = flat[4].clamp(-1e38 / C, 1e38 / C), torch.where(torch.arange(C) % 2 == 0, 1e38 / C, -1e38 / C)
+    x = back(flat.to(t))
+    v, xh, r = O.channel_norm(x, w, b)
+    big = 1 + xh.abs().amax(1, keepdim=True) + x.double().abs().amax(1, keepdim=True) * r
+    for relu in (False, True):
+        leaves = [z.to(dev).requires_grad_() for z in (x, w, b)]
+        gy, a = ops.channel_norm8(*leaves, relu=relu)
+        q, e, rstd, _, _ = gy.grad_fn.saved_tensors
+        want = torch.relu(v) if relu else v
+        assert ((gy.detach().cpu().double() - want).abs() <= half * want.abs() + 2 * F32 * big * (1 + O._ch(w, x).abs())).all()
+        kept, scale = O.values(q.cpu(), e.cpu()), torch.exp2(e.cpu().double() - 127).unsqueeze(1)
+        assert ((kept - xh).abs() <= (1.0 if relu else 0.5) * scale * (1 + 1e-6) + F32 * big).all()
+        assert all(torch.isfinite(g).all() for g in torch.autograd.grad(gy, leaves, dy.to(dev)))
+    flat[5] = torch.finfo(t).max
+    gy, a = ops.channel_norm8(back(flat.to(t)).to(dev), w.to(dev), b.to(dev), relu=True)
+    hit = (back(flat) == back(flat)[0, 0].new_tensor(torch.finfo(t).max)).all(1, keepdim=True).expand(shape)
+    assert torch.isnan(gy.cpu()[hit]).all() and torch.isnan(ops.restore8(a).cpu()[hit]).all()
+    assert torch.isfinite(gy.cpu()[~hit]).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rms_norm8_where_value_times_weight_leaves_float32(hific, dev, shape, fmt):
+    """y = (x r) w is of ordinary size, x w is not: above 2^128 for values of 1e38 with weights of 1e3, below 2^-126 for values of 1e-20
+    with weights of 1e-25 (and an eps of 1e-36).  Steps are those of y."""
+    from hific_amd import ops
+    flat, back = _tokens(_rand(shape, 31))
+    for size, weight, eps in ((1e37, 1e3, 1e-6), (1e-20, 1e-25, 1e-36)):
+        x, w = back(flat * size), weight * (1 + 0.3 * _rand((shape[1],), 32))
+        xd = x.double()
+        y = xd / torch.sqrt((xd * xd).mean(1, keepdim=True) + eps) * O._ch(w, x)
+        a = ops.rms_norm8(x.to(dev), w.to(dev), eps=eps, fmt=fmt)
+        got, e = ops.restore8(a, torch.float32).cpu().double(), a.e.cpu().double() - 127
+        amax = y.abs().amax(1)
+        assert (amax <= O.QMAX[fmt] * torch.exp2(e) * (1 + F32)).all() and (amax > O.QMAX[fmt] * torch.exp2(e - 1) * (1 - F32)).all()
+        s = torch.exp2(e).unsqueeze(1)
+        half = 0.5 * s if fmt == "int8" else torch.exp2(torch.floor(torch.log2((y.abs() / s).clamp_min(2.0 ** -6)))) * 2.0 ** -4 * s
+        assert ((got - y).abs() <= half * (1 + 1e-6) + F32 * y.abs()).all()
