@@ -319,19 +319,29 @@ static inline TileCfg tile_pick(long long N, int C, int HW, int most, int bytes)
     const TileCfg t = tile_waves(N, C, HW, most, bytes, 4);
     return t.lpx == 0 || (t.lpx * 8 * bytes < 128 && C > 32 * most) ? tile_waves(N, C, HW, most, bytes, 8) : t;
 }
-// F(LPX, CPT, NW) for the configuration t
-#define TILE_DISPATCH(t, MOST, F)                                                                                         \
+// What tile_pick can return (channels per thread as the class 1, 2, 4 or 8 that holds them).  Four waves with pieces of less than 128
+// bytes: at most 32 * most channels.  Eight waves: more than 32 * most channels, and at most twice the width that four waves are left
+// for - where eight of a width have enough workgroups, four of half of it have them too.
+constexpr bool tile_used(int lpx, int cpt, int nw, int most, int bytes) {
+    const int least = cpt <= 2 ? cpt : cpt / 2 + 1;
+    if (nw == 4) return lpx * 8 * bytes >= 128 || least <= (most * lpx > 8 ? most * lpx / 8 : 1);
+    return lpx * bytes <= 16 && cpt >= most * lpx / 16 + 1;
+}
+// F(LPX, CPT, NW) for the configuration t of elements of type T; only the kernels that tile_pick can ask for are built
+#define TILE_DISPATCH(t, T, MOST, F)                                                                                      \
     do {                                                                                                                  \
         if ((t).nw == 8) {                                                                                                \
-            if ((t).lpx == 8) { TILE_CPT(8, t, MOST, F, 8); } else if ((t).lpx == 4) { TILE_CPT(4, t, MOST, F, 8); }      \
-            else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F, 8); } else { TILE_CPT(1, t, MOST, F, 8); }                   \
-        } else if ((t).lpx == 32) { TILE_CPT(32, t, MOST, F, 4); } else if ((t).lpx == 16) { TILE_CPT(16, t, MOST, F, 4); } \
-        else if ((t).lpx == 8) { TILE_CPT(8, t, MOST, F, 4); } else if ((t).lpx == 4) { TILE_CPT(4, t, MOST, F, 4); }     \
-        else if ((t).lpx == 2) { TILE_CPT(2, t, MOST, F, 4); } else { TILE_CPT(1, t, MOST, F, 4); }                       \
+            if ((t).lpx == 8) { TILE_CPT(8, t, T, MOST, F, 8); } else if ((t).lpx == 4) { TILE_CPT(4, t, T, MOST, F, 8); } \
+            else if ((t).lpx == 2) { TILE_CPT(2, t, T, MOST, F, 8); } else { TILE_CPT(1, t, T, MOST, F, 8); }             \
+        } else if ((t).lpx == 32) { TILE_CPT(32, t, T, MOST, F, 4); } else if ((t).lpx == 16) { TILE_CPT(16, t, T, MOST, F, 4); } \
+        else if ((t).lpx == 8) { TILE_CPT(8, t, T, MOST, F, 4); } else if ((t).lpx == 4) { TILE_CPT(4, t, T, MOST, F, 4); } \
+        else if ((t).lpx == 2) { TILE_CPT(2, t, T, MOST, F, 4); } else { TILE_CPT(1, t, T, MOST, F, 4); }                 \
     } while (0)
-#define TILE_CPT(LPX, t, MOST, F, NW)                                                                                     \
-    if ((t).cpt <= 1) { F(LPX, 1, NW); } else if ((t).cpt <= 2) { F(LPX, 2, NW); } else if ((t).cpt <= 4) { F(LPX, 4, NW); } \
-    else { F(LPX, ((MOST) < 8 ? 4 : 8), NW); }
+#define TILE_CPT(LPX, t, T, MOST, F, NW)                                                                                  \
+    if ((t).cpt <= 1) { TILE_ONE(LPX, 1, NW, T, MOST, F) } else if ((t).cpt <= 2) { TILE_ONE(LPX, 2, NW, T, MOST, F) }     \
+    else if ((t).cpt <= 4) { TILE_ONE(LPX, 4, NW, T, MOST, F) } else { TILE_ONE(LPX, ((MOST) < 8 ? 4 : 8), NW, T, MOST, F) }
+#define TILE_ONE(LPX, CPT, NW, T, MOST, F)                                                                                \
+    if constexpr (tile_used(LPX, CPT, NW, MOST, sizeof(T))) { F(LPX, CPT, NW); } else return HIFIC_ERR_UNSUPPORTED;
 // sum / maximum over the waves' results of a tile position
 template <int NW, int TP> __device__ __forceinline__ float waves_sum(const float (*red)[TP], int i) {
     float s = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);

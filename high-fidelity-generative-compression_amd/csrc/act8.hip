@@ -182,7 +182,7 @@ int pack_launch(const T* x, u8_t* q, u8_t* qe, int N, int C, int HW, hipStream_t
                 const long long at = n0 * C * HW;
                 const unsigned blocks = (unsigned)(t.tiles * n);
 #define TILE(LPX, CPT, NW) hipLaunchKernelGGL((act8_pack_tile_kernel<T, FMT, LPX, CPT, NW>), dim3(blocks), dim3(64 * NW), 0, st, x + at, q + at, qe + n0 * HW, C, HW, t.tiles, blocks)
-                TILE_DISPATCH(t, 8, TILE);
+                TILE_DISPATCH(t, T, 8, TILE);
 #undef TILE
                 return hific_launch_status();
             });

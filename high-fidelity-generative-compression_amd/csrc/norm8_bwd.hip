@@ -384,7 +384,7 @@ int norm8_bwd_launch(NormBwd& p, int N, float* d0, float* d1, float* d2, int acc
         const unsigned pit = norm8_pit(t);
         p.tokens = t.blocks;
 #define BWD(LPX, CPT, NW) hipLaunchKernelGGL((norm8_bwd_tile_kernel<T, MODE, SRC, LPX, CPT, NW>), dim3((unsigned)rows), dim3(64 * NW), 0, st, p, (unsigned)rows, pit)
-        TILE_DISPATCH(t, tile_most<T>(), BWD);
+        TILE_DISPATCH(t, T, tile_most<T>(), BWD);
 #undef BWD
     } else if (r.l) {
         if constexpr (MODE == M_RMS) {

@@ -390,7 +390,7 @@ int norm8_fwd_launch(NormFwd& p, int N, hipStream_t st) {
                     if (p.resid) hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, true, LPX, CPT, NW>), grid, dim3(64 * NW), 0, st, part, grid.x); \
                     else hipLaunchKernelGGL((norm8_fwd_tile_kernel<T, MODE, FMT, false, LPX, CPT, NW>), grid, dim3(64 * NW), 0, st, part, grid.x); \
                 } while (0)
-                TILE_DISPATCH(t, tile_most<T>(), FWD);
+                TILE_DISPATCH(t, T, tile_most<T>(), FWD);
 #undef FWD
                 return hific_launch_status();
             });
