@@ -219,7 +219,7 @@ int restore_launch(const u8_t* q, const u8_t* qe, const float* gamma, const floa
         });
     }
     constexpr int CH = 4;
-    const unsigned octs = HW >= 8 ? (unsigned)cdiv(HW, 8) : (unsigned)HW, cgs = (unsigned)cdiv(C, CH);
+    const unsigned octs = HW >= 8 ? (unsigned)cdivl(HW, 8) : (unsigned)HW, cgs = (unsigned)cdiv(C, CH);
     const long long each = (long long)octs * cgs;                     // threads of an image
     if (cdivl(each, 256) >= 1ll << 24) return HIFIC_ERR_UNSUPPORTED;  // (an image of more than 10^11 values)
     return batch_parts(N, cdivl(each, 256), [&](long long n0, long long n) {

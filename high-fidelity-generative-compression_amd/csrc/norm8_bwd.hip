@@ -360,7 +360,7 @@ size_t norm8_rows(int mode, int N, int C, int HW) {
     if (mode == M_RMS && HW == 1 && C >= 8) {
         const RowCfg r = row_pick(N, C);
         if (r.l) {                       // at least four groups of rows per workgroup once every CU has one: each writes a row of C sums
-            const int g = cdiv(N, row_block(r.l) / r.l);
+            const int g = (int)cdivl(N, row_block(r.l) / r.l);
             return (size_t)(g <= 256 ? g : (g < 1024 ? 256 : (g < 4096 ? cdiv(g, 4) : 1024)));
         }
     }

@@ -49,3 +49,14 @@ def test_tiles_that_are_built_are_those_that_shapes_ask_for(tmp_path):
     subprocess.check_call([hipcc, "--offload-arch=gfx950", "--offload-host-only", "-O1", "-std=c++17", "-I" + os.path.join(g.PKG, "csrc"), str(src), "-o", str(exe)],
                           stderr=subprocess.DEVNULL)
     assert subprocess.run([str(exe)], stdout=subprocess.PIPE, text=True).stdout.strip() == "ok"
+
+
+def test_counts_near_32_bits(hific):
+    """Rows up to 2^31 - 1: the workspace of the backward pass stays the one of a little fewer."""
+    from hific_amd import lib
+    ws = lib.raw("hific_norm8_bwd_ws_bytes")
+    for c in (8, 64, 129, 960, 4096, 16384):
+        want = ws(2 ** 31 - 2000, c, 1)
+        assert 0 < want < 1 << 30
+        for n in (2 ** 31 - 33, 2 ** 31 - 31, 2 ** 31 - 9, 2 ** 31 - 1):
+            assert ws(n, c, 1) == want, (n, c)
