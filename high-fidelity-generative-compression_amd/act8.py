@@ -352,6 +352,18 @@ def _cn8_bwd(q, e, rstd, dy, gamma, beta, relu, dg, db, acc, dprev=None, acc_pre
     return dx
 
 
+def _norm_targets(want, g_slot, gamma, b_slot, beta):
+    """(tensors to write for gamma and beta, accumulate flag, values to return to autograd).  The kernel has one flag for both: where one
+    of them is added to and the other is written for the first time (one in an arena, one not), the other starts from zeros."""
+    if not want:
+        return torch.empty_like(gamma), torch.empty_like(beta), 0, None, None
+    dgt, acc_g, dg = ops._grad_target(g_slot, gamma)
+    dbt, acc_b, db = ops._grad_target(b_slot, beta)
+    if acc_g != acc_b:
+        (dbt if acc_g else dgt).zero_()
+    return dgt, dbt, acc_g | acc_b, dg, db
+
+
 class ChannelNorm8Fn(Function):
     """ChannelNormFn whose backward pass reads the normalised activation in 8 bits."""
 
@@ -374,9 +386,7 @@ class ChannelNorm8Fn(Function):
         q, e, rstd, gamma, beta = ctx.saved_tensors
         dy = c16(dy)
         want = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dgt, acc, dg = ops._grad_target(ctx.g_slot, gamma) if want else (torch.empty_like(gamma), 0, None)
-        dbt, acc_b, db = ops._grad_target(ctx.b_slot, beta) if want else (torch.empty_like(beta), 0, None)
-        assert acc == acc_b
+        dgt, dbt, acc, dg, db = _norm_targets(want, ctx.g_slot, gamma, ctx.b_slot, beta)
         dx = _cn8_bwd(q, e, rstd, dy, gamma, beta, ctx.relu, dgt, dbt, acc)
         if want:
             ops._written(ctx.g_slot, ctx.b_slot)
@@ -576,9 +586,7 @@ class ConvNorm8Fn(Function):
         need = ctx.needs_input_grad
         with _on(dy):
             want_n = need[9] or need[10]
-            dgt, acc_g, dg = ops._grad_target(ctx.g_slot, gamma) if want_n else (torch.empty_like(gamma), 0, None)
-            dbt, acc_b, dbe = ops._grad_target(ctx.be_slot, beta) if want_n else (torch.empty_like(beta), 0, None)
-            assert acc_g == acc_b
+            dgt, dbt, acc_g, dg, dbe = _norm_targets(want_n, ctx.g_slot, gamma, ctx.be_slot, beta)
             want_b = ctx.has_bias and need[7]
             dpt, acc_p, db = ops._grad_target(ctx.b_slot, gamma.new_empty(gamma.numel())) if want_b else (None, 0, None)
             dz = _cn8_bwd(nq, ne, rstd, dy, gamma, beta, ctx.relu, dgt, dbt, acc_g, dpt, acc_p)

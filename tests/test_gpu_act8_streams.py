@@ -72,3 +72,36 @@ def test_an_input_whose_norm_parameters_are_temporaries(hific, dev):
     assert torch.isfinite(res[0][0]).all()
     for s, t in zip(*res):
         assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("block", [False, True])
+@pytest.mark.parametrize("in_arena", ["gamma", "beta", "both"])
+def test_a_norm_with_one_parameter_in_an_arena(hific, dev, in_arena, block):
+    """The second backward pass adds to the arena's gradient and hands the other one to autograd."""
+    from hific_amd import ops, optim
+    from hific_amd.network.layers import HipConv2d
+    from hific_amd.normalisation.channel import ChannelNorm2D, fuse_bias_grad
+    C = 32
+    x = _rand((2, C, 12, 12), 21, torch.bfloat16).to(dev)
+    dys = [_rand((2, C, 12, 12), 22 + i, torch.bfloat16).to(dev) for i in range(3)]
+    torch.manual_seed(9)
+    conv = HipConv2d(C, C, 3, stride=1, pads=(1, 1, 1, 1)).to(dev)
+    start = ChannelNorm2D(C, fuse_relu=True).to(dev).state_dict()
+
+    def run(members, n):
+        norm = ChannelNorm2D(C, fuse_relu=True).to(dev)
+        norm.load_state_dict(start)
+        fuse_bias_grad(conv, norm)
+        if members:
+            optim.ParamArena([getattr(norm, m) for m in members])
+        for dy in dys[:n]:
+            xd = x.clone().requires_grad_()
+            y = ops.conv_norm8(xd, ops.checkpoint8(x), conv, norm)[0] if block else ops.channel_norm8(xd, norm.gamma, norm.beta, relu=True)[0]
+            y.backward(dy)
+        torch.cuda.synchronize()
+        return norm.gamma.grad.clone(), norm.beta.grad.clone()
+    members = ["gamma", "beta"] if in_arena == "both" else [in_arena]
+    for n in (1, 2, 3):
+        for got, want in zip(run(members, n), run([], n)):
+            # float32 sums of the same terms; the arena's is formed inside the kernel, autograd's outside
+            assert float((got - want).abs().max()) <= 4 * 2.0 ** -24 * n * 288 * 4
