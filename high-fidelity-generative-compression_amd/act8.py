@@ -137,10 +137,22 @@ def _first_order(backward):
     return run
 
 
+def _arena(t):
+    slot = ops._slot(t)
+    return None if slot is None else slot.arena
+
+
+def _token(t, arena):
+    """Changes with the values of a parameter: torch counts writes in place (not of inference tensors), an arena its optimizer's steps."""
+    return 0 if t.is_inference() else t._version, 0 if arena is None else arena.epoch
+
+
 class Act8:
-    """An activation in 8 bits: `q` (int8 or float8_e4m3fn) [N, C, ...] and `e` (uint8, exponent + 127) [N, ...].  With `gamma` /
-    `beta` (float32, C values) it stands for relu?(gamma * (q * 2^e) + beta): a norm's output held as its normalised values."""
-    __slots__ = ("q", "e", "gamma", "beta", "relu")
+    """An activation in 8 bits: `q` (int8 or float8_e4m3fn) [N, C, ...] and `e` (uint8, exponent + 127, from 1 on) [N, ...].  With `gamma` /
+    `beta` (float32, C values) it stands for relu?(gamma * (q * 2^e) + beta): a norm's output held as its normalised values.  It holds
+    these tensors themselves, not copies: one that channel_norm8 or conv_norm8 returned stands for their output until its norm's
+    parameters change (an optimizer step), and is refused from then on."""
+    __slots__ = ("q", "e", "gamma", "beta", "relu", "_made")
 
     def __init__(self, q, e, gamma=None, beta=None, relu=False):
         if q.dtype not in _CODE or e.dtype != torch.uint8:
@@ -154,14 +166,27 @@ class Act8:
         for t, name in ((gamma, "gamma"), (beta, "beta")):
             if t is not None:
                 _param(t, C, name)
-        self.q, self.e, self.gamma, self.beta, self.relu = c16(q), c16(e), gamma, beta, bool(relu)
+        self.q, self.e, self.gamma, self.beta, self.relu, self._made = c16(q), c16(e), gamma, beta, bool(relu), None
 
     @classmethod
     def _of(cls, q, e, gamma=None, beta=None, relu=False):
-        """Without the checks: tensors that were just made."""
+        """Without the checks: tensors that were just made; gamma and beta a norm's parameters."""
         a = object.__new__(cls)
-        a.q, a.e, a.gamma, a.beta, a.relu = q, e, gamma, beta, relu
+        a.q, a.e, a.relu = q, e, relu
+        if gamma is None:
+            a.gamma = a.beta = a._made = None
+        else:
+            a.gamma, a.beta = g, b = gamma.detach(), beta.detach()       # (the same version counters)
+            ga, ba = _arena(gamma), _arena(beta)
+            a._made = ga, _token(g, ga), ba, _token(b, ba)
         return a
+
+    def _current(self):
+        """Refuses values of a norm whose parameters have changed since."""
+        m = self._made
+        if m is not None and (_token(self.gamma, m[0]) != m[1] or _token(self.beta, m[2]) != m[3]):
+            raise lib.HificError("this Act8 holds a norm's output as its normalised values, and the norm's gamma or beta have changed since")
+        return self
 
     @property
     def fmt(self):
@@ -203,6 +228,7 @@ def restore8(a, dtype=torch.bfloat16):
         raise lib.HificError(f"restore8 needs an Act8, got {type(a).__name__}")
     if dtype not in (torch.float32, torch.bfloat16):
         raise lib.HificError(f"restore8: dtype must be torch.float32 or torch.bfloat16, not {dtype}")
+    a._current()
     return _restore(a.q, a.e, a.gamma, a.beta, a.relu, dtype)
 
 
@@ -418,7 +444,7 @@ def channel_norm8(x, gamma, beta, eps=1e-3, relu=False, resid=None, fmt="int8"):
     y, q, e = ChannelNorm8Fn.apply(c16(x), gamma, beta, _eps(eps), bool(relu), resid, geom, cd, code, dt)
     if resid is not None:
         return y, Act8._of(q, e)
-    return y, Act8._of(q, e, gamma.detach(), beta.detach(), bool(relu))
+    return y, Act8._of(q, e, gamma, beta, bool(relu))
 
 
 def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
@@ -611,7 +637,7 @@ def conv_norm8(x, x8, conv, norm, resid=None, fmt="int8"):
                                 bool(norm.fuse_relu), None if resid is None else c16(resid), code, dt)
     if resid is not None:
         return y, Act8._of(q, e)
-    return y, Act8._of(q, e, norm.gamma.detach(), norm.beta.detach(), bool(norm.fuse_relu))
+    return y, Act8._of(q, e, norm.gamma, norm.beta, bool(norm.fuse_relu))
 
 
 def _split8(x8, x):
@@ -620,6 +646,7 @@ def _split8(x8, x):
     if not isinstance(x8, Act8) or x8.shape != x.shape:
         raise lib.HificError(f"x8 must be the Act8 of x {tuple(x.shape)}")
     _one_device(x, x8.q)
+    x8._current()
     return x8.q, x8.e, x8.gamma, x8.beta, x8.relu
 
 
@@ -723,6 +750,7 @@ def _conv_wgrad8(saved, relu, dy, dw, acc, geom, cd, own_ws=False):
 def _wgrad_args(a, dy, kernel, name):
     if not isinstance(a, Act8) or a.q.dim() != 4:
         raise lib.HificError(f"{name} needs a 4-dimensional Act8")
+    a._current()
     if dy.dim() != 4 or dy.shape[0] != a.shape[0] or dy.shape[1] < 1:
         raise lib.HificError(f"{name}: dy must be [{a.shape[0]}, K, OH, OW], got {tuple(dy.shape)}")
     R, S = (int(k) for k in kernel)
