@@ -449,7 +449,7 @@ def channel_norm8(x, gamma, beta, eps=1e-3, relu=False, resid=None, fmt="int8"):
 
 def channel_norm_grad8(a, dy, gamma, beta, rstd, relu=False):
     """(dx, dgamma, dbeta) of channel_norm8 from what its forward pass kept: `a` the normalised values (q, e), `rstd` float32
-    [N, ...] the reciprocal standard deviations, dy float32 or bfloat16."""
+    [N, ...] the reciprocal standard deviations, dy float32 or bfloat16.  Carries no gradient."""
     if not isinstance(a, Act8) or a.gamma is not None:
         raise lib.HificError("channel_norm_grad8 needs the normalised values as an Act8 without gamma / beta")
     geom = _norm_args(a.q, gamma, beta, "channel_norm_grad8")
@@ -473,7 +473,10 @@ if _CHECKPOINT8 is not None:
 
 
 def set_checkpoint8(fmt):
-    """"int8" | "e4m3": training forwards keep 8-bit activations (see above); None: bfloat16 / float32 ones."""
+    """"int8" | "e4m3": training forwards keep 8-bit activations (see above); None: bfloat16 / float32 ones.  Where it acts: the Generator's
+    fused conv -> ChannelNorm chain, and the Encoder's with set_exact_index(False).  Everything else keeps what it kept: the exact chains
+    (set_exact_training, set_exact_reconstruction, set_exact_index), instance norms, a Generator that samples noise, the hyperprior and
+    the Discriminator."""
     global _CHECKPOINT8
     if fmt is not None:
         _fmt(fmt)
@@ -764,7 +767,7 @@ def _wgrad_args(a, dy, kernel, name):
 def conv2d_weight_grad8(a, dy, kernel, stride=1, pads=(0, 0, 0, 0), pad_mode=lib.PAD_ZERO):
     """Weight gradient [K, C, R, S] (float32) of conv2d whose input is held as `a`, dy [N, K, OH, OW] float32 or bfloat16: what
     conv2d's backward pass gives for restore8(a, dy.dtype).  In bfloat16 the restored values of a plain Act8 are exact, so the
-    products are exact and the sum is float32."""
+    products are exact and the sum is float32.  Carries no gradient."""
     R, S, dy = _wgrad_args(a, dy, kernel, "conv2d_weight_grad8")
     N, C, H, W = a.shape
     pt, pl, pb, pr = (int(v) for v in pads)

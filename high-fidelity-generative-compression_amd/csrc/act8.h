@@ -4,11 +4,15 @@
 // A token is one position of an activation [N, C, HW]; its C values share ONE exponent.  q is int8 or e4m3 (finite-only,
 // largest value 448), shape of the tensor; qe [N, HW] holds exponent + 127 in a byte:
 //     value = q * 2^(qe - 127),   qe = smallest exponent with max|v| <= QMAX * 2^(qe - 127),  QMAX = 127 or 448
-// Powers of two, not max|v| / QMAX: q * 2^e then has at most 8 significant bits, so a restored value is EXACT in bfloat16 and a
+// Powers of two, not max|v| / QMAX: q * 2^e then has at most 8 significant bits, so a restored value is EXACT in bfloat16 (down to
+// 2^-133) and a
 // product over restored values carries the one rounding of q and no second one; the price is up to one bit of int8's range
 // (e4m3 loses nothing: it has its own exponent).  qe = 255 marks a token with an infinity or NaN: it restores to NaN as a
 // whole, so that a diverged activation never comes back finite; a finite token comes back finite (q8_top).  A token of zeros has
 // qe = 1 (2^-126).
+//
+// Times in the comments of these files: one MI355X, bfloat16 unless said, calls of the C entry point back to back (launches and, in a
+// backward pass, the column sums included), three sets of operands in turn; variants that are set against each other ran side by side.
 #pragma once
 #include "common.h"
 
@@ -163,7 +167,7 @@ __device__ __forceinline__ u32x2_t q8_pack8(const float* t) {
     return o;
 }
 // byte B of u, signed, as a number: one instruction (a sub-dword operand with sign extension; written out because the compiler extends
-// bytes that are used in two places in one of their own first: rows of 960 from int8, backward 65 us with it, 69 without)
+// bytes that are used in two places in one of their own first: rows of 960 from int8, backward 67 us with it, 69 without)
 template <int B>
 __device__ __forceinline__ float byte_f32(unsigned u) {
     float v;
@@ -381,7 +385,7 @@ template <int L> __device__ __forceinline__ float row_sum(float v) { return row_
 template <int L> __device__ __forceinline__ unsigned row_max(unsigned v) { return row_reduce<L>(v, [](unsigned a, unsigned b) { return umax(a, b); }); }
 // As few lanes of a wave as hold the row in one group each (65536x129, both passes: 32 lanes 36 us, 64 lanes 52), the wave with up to 4 groups for
 // wider ones, a workgroup of 256 above 2048 channels and where fewer than 1024 rows would leave the other CUs idle, one of 1024
-// threads above 8192 (2048x16384, both passes: 126 us, the any-shape kernels 331).  l = 0: more channels than the registers hold.
+// threads above 8192 (2048x16384, both passes: 130 us, the any-shape kernels 331).  l = 0: more channels than the registers hold.
 struct RowCfg { int l, k; };
 static inline RowCfg row_pick(long long N, int C) {
     RowCfg r;

@@ -1,10 +1,10 @@
 // Activation checkpoints in 8 bits (format: act8.h): pack an activation, restore it.  Both are bound by HBM: pack reads T and
-// writes 1 byte per element, restore the reverse.  bfloat16, us (TB/s): 16x60x256x256 pack 39 (4.8), restore 40 (4.7); 16x240x64x64 9.6
-// (4.9) both; 16x960x16x16 4.8 (2.4) both, half of it the launch.
+// writes 1 byte per element, restore the reverse.  us (TB/s): 16x60x256x256 pack 38.6 (4.9), restore 34.7 (5.4), with
+// gamma, beta and ReLU 40.4 (4.7); 16x240x64x64 10.1 (4.7), 8.6 (5.5), 9.7; 16x960x16x16 4.8, 4.9, 5.2, most of it the launch.
 #include "act8.h"
 
-// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor read twice (the second time from L2; 2x3000x32x32
-// 115 us, which the tiles below take in 10: a few workgroups with long chains of loads).
+// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor read twice (the second time from L2).  A few
+// workgroups with long chains of loads: 16x960x2x2 17 us, 2x4500x16x16 120 (2x3000x32x32 115, which the tiles below take in 10).
 template <typename T, int FMT, int PX>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                         int C, int HW, long long tokens) {
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* __restrict__ x,
 }
 
 // Planes of eight positions and more: the tile stays in registers between the maximum and the rounding, one pass over HBM (3x220x45x31
-// 3.7 us against a floor of 0.5: latency).
+// 4.4 us against a floor of 0.5: the launch and latency).
 template <typename T, int FMT, int LPX, int CPT, int NW>
 __global__ __launch_bounds__(64 * NW) void act8_pack_tile_kernel(const T* __restrict__ x, u8_t* __restrict__ q, u8_t* __restrict__ qe,
                                                              int C, int HW, unsigned tiles, unsigned blocks) {

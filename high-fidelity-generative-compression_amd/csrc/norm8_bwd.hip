@@ -83,9 +83,9 @@ __global__ __launch_bounds__(256) void norm8_param_kernel(const NormBwd p) {
 
 // Planes: as norm8_fwd_tile_kernel.  A workgroup takes `pit` tiles in turn (p.tokens counts tiles here) and keeps the sums of its
 // channels in registers: part[workgroup][0..2][c] as norm8_param_kernel.  Bound by the issue of its instructions as much as by HBM (about
-// 20 per value: two unpackings, mask, two sums, three channel sums; registers allow eight waves per CU).  bfloat16, us (TB/s): channel
-// norm + ReLU from int8 16x60x256x256 80 (3.9), 16x120x128x128 37 (4.2), 16x960x16x16 8.5 (2.3); root-mean-square norm with the stream's
-// gradient 114 (4.4), 55 (4.6), 9.5 (3.3).
+// 20 per value: two unpackings, mask, two sums, three channel sums; registers allow eight waves per CU).  us (TB/s): channel
+// norm + ReLU from int8 16x60x256x256 83.6 (3.8), 16x120x128x128 42.5 (3.7), 16x960x16x16 12.3 (1.6); root-mean-square norm with the stream's
+// gradient 115.7 (4.3), 58.7 (4.3), 13.2 (2.4), from int8 without it 83.6, 43.3, 11.8.
 template <typename T, int MODE, int SRC, int LPX, int CPT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void norm8_bwd_tile_kernel(const NormBwd p, unsigned blocks, unsigned pit) {
     constexpr int SUBS = 64 / LPX, G = NW * SUBS, TP = LPX * 8;
@@ -206,8 +206,8 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_bwd_tile_kernel(const NormBw
     }
 }
 
-// Rows: a workgroup takes every gridDim.x-th group of R rows and keeps the sums of its channels in registers.  65536x960 bfloat16 110 us
-// (4.6 TB/s), 16384x4096 120 us (4.5).
+// Rows: a workgroup takes every gridDim.x-th group of R rows and keeps the sums of its channels in registers.  65536x960 104 us
+// (4.8 TB/s), 16384x4096 115 us (4.7); from int8 without the stream's gradient 68 and 79.
 template <typename T, int SRC, int L, int K>
 __global__ __launch_bounds__(row_block(L)) void rms_bwd_rows_kernel(const NormBwd p, int N) {
     constexpr int R = row_block(L) / L;
@@ -302,8 +302,8 @@ __global__ __launch_bounds__(row_block(L)) void rms_bwd_rows_kernel(const NormBw
 }
 
 // column sums of part[rows][nr * C] into up to three vectors, each written or added to, in a fixed order: 16 columns x 64 row
-// lanes per workgroup (a few hundred columns of ~1000 rows: more row lanes, so that no thread adds more than a few dozen).  3.4 us,
-// the launch, for 512 rows of 480 sums; 12 for 1024 of 16384.
+// lanes per workgroup (a few hundred columns of ~1000 rows: more row lanes, so that no thread adds more than a few dozen).  As a launch
+// of its own about 4 us for 512 rows of 480 sums; 12 for 1024 of 16384.
 __global__ __launch_bounds__(1024) void norm8_colsum_kernel(const float* __restrict__ part, float* __restrict__ d0, float* __restrict__ d1,
                                                             float* __restrict__ d2, int C, int rows, int nr, int acc, int acc2) {
     __shared__ float red[64][17];

@@ -23,8 +23,8 @@ __device__ __forceinline__ float norm8_r(float ss, float nv, float eps) { return
 // max|d w| r does not give the exponent of y = (d r) w where d * w left the range of float32 or lost its bits below it
 __device__ __forceinline__ bool norm8_far(float m, float ss) { return m == INFINITY || (m < 0x1p-100f && ss > 0.f); }
 
-// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2; 2x3000x32x32 250 us, which
-// the tiles below take in 17).
+// Any shape: PX lanes on consecutive tokens x 256 / PX channel groups, the tensor re-read by every pass (from L2).  Chains of loads
+// bound it: channel norm 16x960x2x2 39 us, 16x960x2x3 44, 2x4500x16x16 232 (2x3000x32x32 250, which the tiles below take in 17).
 template <typename T, int MODE, int FMT, int PX>
 __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long long tokens) {
     constexpr int G = 256 / PX;
@@ -102,9 +102,10 @@ __global__ __launch_bounds__(256) void norm8_fwd_kernel(const NormFwd p, long lo
 }
 
 // Planes of eight positions and more: a workgroup owns LPX * 8 positions x all channels (tile_pick), eight positions and CPT
-// channels per lane, kept as they were loaded between the passes: every tensor crosses HBM once, and that bounds it.  bfloat16, us (TB/s): channel
-// norm + ReLU 16x60x256x256 70 (4.5), 16x120x128x128 38 (4.1), 16x960x16x16 8.6 (2.3: the latency of three dependent passes);
-// root-mean-square norm with residual 105 (4.8), 56 (4.5), 8.5 (3.7).
+// channels per lane, kept as they were loaded between the passes: every tensor crosses HBM once, and that bounds it.  us (TB/s): channel
+// norm + ReLU 16x60x256x256 70.5 (4.5), 16x120x128x128 38.6 (4.1), 16x960x16x16 8.8 (2.2: the latency of three dependent passes), with
+// a residual and its second 8-bit form 107.6 (4.7), 52.4 (4.8), 11.5 (2.7); root-mean-square norm with residual 108.1 (4.7), 53.4 (4.7),
+// 8.8 (3.6), with its normalised form kept 122.6 (4.6), 62.9 (4.5), 10.4 (3.4).
 template <typename T, int MODE, int FMT, bool RES, int LPX, int CPT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFwd p, unsigned blocks) {
     constexpr int SUBS = 64 / LPX, G = NW * SUBS, TP = LPX * 8;
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(64 * NW, 2) void norm8_fwd_tile_kernel(const NormFw
 }
 
 // Rows of eight channels and more (root-mean-square norm): eight channels per lane, L lanes and K groups per lane for a row.  65536x960
-// bfloat16 with residual 78 us (6.5 TB/s: part of it from the memory-side cache), 16384x4096 90 us (6.0), one row 2.2 us (the launch).
+// with residual 87 us (5.8 TB/s: part of it from the memory-side cache), 16384x4096 94 us (5.7), to 8 bits 38 and 40; one row 4.9 us (the launch).
 template <typename T, int FMT, int L, int K>
 __global__ __launch_bounds__(row_block(L)) void rms_fwd_rows_kernel(const NormFwd p, int N) {
     constexpr int F = FMT == Q_NONE ? HIFIC_Q_INT8 : FMT;

@@ -27,7 +27,7 @@ struct WgTaps {
 // T, eight neighbours of one row (of eight and more) per thread, at the row's end moved back to end with it.  What they are read from
 // lies in one window of eight (stride 2: sixteen) bytes of one input row, reflected columns included: a byte permutation picks them,
 // and only the lanes at a row's ends form its selectors.  Other shapes (narrow rows, large strides or pads), and the ends of bfloat16
-// rows: value by value.  Bound by the latency of its index arithmetic and loads on small planes (2x120x61x47 stride 2: 5.5 us), by its
+// rows: value by value.  Bound by the latency of its index arithmetic and loads on small planes (2x120x61x47 stride 2: 5.3 us), by its
 // instructions on large ones (16x480x32x32 stride 2, 25 MB written: 17 us, value by value 41).
 template <int SRC>
 __global__ __launch_bounds__(256) void wgrad8_taps_kernel(const WgTaps p, bf16_t* __restrict__ out, unsigned total) {
