@@ -181,6 +181,22 @@ class Act8:
             a._made = ga, _token(g, ga), ba, _token(b, ba)
         return a
 
+    @classmethod
+    def _held(cls, *values):
+        a = object.__new__(cls)
+        a.q, a.e, a.gamma, a.beta, a.relu, a._made = *values, None
+        return a
+
+    def __reduce__(self):
+        """Copied and saved with the parameters as they are, which nobody else changes then; not with the arena they live in."""
+        self._current()
+        return Act8._held, (self.q, self.e, self.gamma, self.beta, self.relu)
+
+    def __copy__(self):
+        a = Act8._held(self.q, self.e, self.gamma, self.beta, self.relu)
+        a._made = self._made
+        return a
+
     def _current(self):
         """Refuses values of a norm whose parameters have changed since."""
         m = self._made
