@@ -141,6 +141,7 @@ int hific_channelnorm_bwd(const void* x, const void* dy, const float* gamma, con
  * max|v| <= QMAX * 2^(qe - 127) over the token's C values, QMAX = 127 or 448 (1 <= qe).  qe = 255: the token held an infinity or NaN
  * and restores to NaN.  A finite token restores to finite values: where the nearest value would be 2^128, the one below it is kept.  All tensors contiguous; no alignment is needed.  Planes of eight positions and more (up to 2048 channels;
  * 4096 in bfloat16) and rows (HW = 1) of 8 to 16384 channels cross memory once; other shapes are read two or three times.
+ * A norm's token whose sum of squares leaves float32 is summed again in a wider range; a channel norm's whose plain sum does is NaN.
  * x, y, resid, dy, ... are of `dtype`; weights, statistics and their gradients float32.  At most 2^20 channels in what forms a
  * token's sums or exponent. */
 #define HIFIC_Q_INT8 0
