@@ -448,8 +448,9 @@ def _norm_args(x, gamma, beta, name):
 def channel_norm8(x, gamma, beta, eps=1e-3, relu=False, resid=None, fmt="int8"):
     """channel_norm (src/normalisation/channel.py:48-59, with the ReLU or the residual behind it) -> (y, Act8): y as channel_norm
     gives it (but for a position with an infinity or NaN, which stays NaN behind the ReLU too, and one of values above 1e19, whose
-    squares leave float32: normalised here, zeros there), and the Act8 stands for y too - what the next convolution's weight gradient reads (conv2d(x8=)).  The backward pass of the norm keeps its normalised input in
-    8 bits and nothing else of x or y.  With `relu` the kept values are on the same side of the ReLU as the forward values."""
+    squares leave float32: it is normalised here), and the Act8 stands for y too - what the next convolution's weight gradient reads
+    (conv2d(x8=)).  The backward pass of the norm keeps its normalised input in 8 bits and nothing else of x or y.  With `relu` the
+    kept values are on the same side of the ReLU as the forward values."""
     geom = _norm_args(x, gamma, beta, "channel_norm8")
     code, dt = _fmt(fmt)
     cd = lib.dtype_code(x)
